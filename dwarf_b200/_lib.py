@@ -14,6 +14,7 @@ LIB_PATH = os.path.join(PKG_DIR, "libdsqg_b200.so")
 
 DSQG_DTYPE_BF16 = 0
 DSQG_DTYPE_F32 = 1
+DSQG_DTYPE_E4M3 = 2
 DSQG_MAX_TAPS = 128
 DSQG_STATIC_SCRATCH_BYTES = 8 << 20
 
@@ -87,7 +88,30 @@ _SIGNATURES = {
     "dsqg_ring_prefill_kv": (c_int, [c_void_p] * 5 + [c_int] * 6 + [c_void_p]),
     "dsqg_decode_overlapped": (c_int, [c_void_p] * 3 + [c_void_p] * 2 + [c_void_p] * 2 + [c_void_p] * 3
                                + [POINTER(c_int32), c_int, c_int] + [c_void_p] + [c_int] * 4 + [c_void_p]),
+    "dsqg_rms_norm_fwd": (c_int, [c_void_p] * 2),
+    "dsqg_rms_norm_bwd_scratch_bytes": (c_size_t, [ctypes.c_longlong, c_int]),
+    "dsqg_rms_norm_bwd": (c_int, [c_void_p] * 7 + [c_size_t, c_void_p]),
+    "dsqg_decode_kv_e4m3": (c_int, [c_void_p] * 10 + [POINTER(c_int32), c_int, c_int] + [c_void_p] + [c_int] * 4 + [c_void_p, c_int]),
+    "dsqg_ring_prefill_e4m3": (c_int, [c_void_p] * 6 + [c_int] * 6 + [c_void_p]),
+    "dsqg_dequantize_rows": (c_int, [c_void_p] * 3 + [ctypes.c_longlong, c_int, c_int, c_void_p]),
+    "dsqg_paged_write": (c_int, [c_void_p] * 3 + [ctypes.c_longlong] * 4 + [c_void_p] * 2 + [ctypes.c_longlong, c_int, c_void_p]),
+    "dsqg_paged_read": (c_int, [c_void_p] * 5 + [ctypes.c_longlong, c_int, c_void_p]),
+    "dsqg_paged_step_scratch_bytes": (c_size_t, [c_int] * 5),
+    "dsqg_paged_step": (c_int, [c_void_p] * 5 + [c_int, c_int, c_float] + [c_void_p] * 2 + [c_size_t, c_int, c_void_p]),
+    "dsqg_int4_linear": (c_int, [c_void_p] * 6 + [c_int] * 5 + [c_void_p]),
 }
+
+
+class RmsNorm(ctypes.Structure):
+    """dsqg_rms_norm."""
+    _fields_ = [(n, c_void_p) for n in ("x", "residual", "weight", "h", "y", "y_scale", "rstd")] + [
+        ("rows", ctypes.c_longlong), ("D", c_int), ("eps", c_float), ("x_dtype", c_int), ("stream_dtype", c_int), ("y_dtype", c_int)]
+
+
+class Pages(ctypes.Structure):
+    """dsqg_pages."""
+    _fields_ = [(n, c_void_p) for n in ("kv", "scale", "table")] + [(n, c_int) for n in ("dtype", "sequences", "columns", "pages", "page_size", "heads", "D")]
+
 
 EXPORTED_SYMBOLS = tuple(_SIGNATURES)
 

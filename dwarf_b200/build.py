@@ -13,7 +13,9 @@ CSRC = os.path.join(PKG_DIR, "csrc")
 INCLUDE = os.path.join(os.path.dirname(PKG_DIR), "include")
 LIB_PATH = os.path.join(PKG_DIR, "libdsqg_b200.so")
 EXT_PATH = os.path.join(PKG_DIR, "_dsqg_torch.so")
-SOURCES = ["dsqg_capi.cu", "dsqg_dispatch.cu", "dsqg_generic.cu", "dsqg_decode.cu", "dsqg_mma.cu", "dsqg_mma_d64.cu", "dsqg_mma_window.cu", "dsqg_mma_widths.cu", "dsqg_staged.cu", "dsqg_umma.cu", "dsqg_static.cu", "dsqg_gate.cu", "dsqg_scan.cu", "dsqg_layer.cu", "dsqg_wgrad.cu"]
+SOURCES = ["dsqg_capi.cu", "dsqg_dispatch.cu", "dsqg_generic.cu", "dsqg_decode.cu", "dsqg_mma.cu", "dsqg_mma_d64.cu", "dsqg_mma_window.cu", "dsqg_mma_widths.cu", "dsqg_staged.cu", "dsqg_umma.cu", "dsqg_static.cu", "dsqg_gate.cu", "dsqg_scan.cu", "dsqg_layer.cu", "dsqg_wgrad.cu", "dsqg_norm.cu", "dsqg_decode8.cu",
+           "dsqg_paged.cu", "dsqg_paged_mma.cu", "dsqg_int4.cu"]
+EXT_SOURCES = ["dsqg_torch.cpp", "dsqg_torch_serving.cpp"]
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
               "-Xcompiler", "-fPIC"]
 
@@ -57,9 +59,11 @@ def build_library(force: bool = False, verbose: bool = False) -> str:
     os.makedirs(build_dir, exist_ok=True)
     procs = []
     comp, link_ext = _torch_flags()
-    ext_obj = os.path.join(build_dir, "dsqg_torch.o")
-    jobs = [("dsqg_torch.cpp", ["g++", "-O2", "-std=c++17", "-fPIC", "-fvisibility=hidden", "-I", INCLUDE, *comp,
-                                "-c", os.path.join(CSRC, "dsqg_torch.cpp"), "-o", ext_obj])]
+    ext_objs, jobs = [], []
+    for src in EXT_SOURCES:
+        ext_objs.append(os.path.join(build_dir, src.replace(".cpp", ".o")))
+        jobs.append((src, ["g++", "-O2", "-std=c++17", "-fPIC", "-fvisibility=hidden", "-I", INCLUDE, *comp,
+                           "-c", os.path.join(CSRC, src), "-o", ext_objs[-1]]))
     for src in SOURCES:
         obj = os.path.join(build_dir, src.replace(".cu", ".o"))
         cmd = [nvcc, *NVCC_FLAGS, "-I", INCLUDE, "-I", CSRC, "-c", os.path.join(CSRC, src), "-o", obj]
@@ -78,7 +82,7 @@ def build_library(force: bool = False, verbose: bool = False) -> str:
         if p.returncode != 0:
             raise RuntimeError(f"compiling {src} failed:\n{out}")
     subprocess.check_call([nvcc, "-shared", "-o", LIB_PATH, *objs, "-gencode", "arch=compute_100a,code=sm_100a", "-lcudart", "-ldl"])
-    subprocess.check_call(["g++", "-shared", "-o", EXT_PATH, ext_obj, "-L", PKG_DIR, "-ldsqg_b200", "-Wl,-rpath,$ORIGIN", *link_ext])
+    subprocess.check_call(["g++", "-shared", "-o", EXT_PATH, *ext_objs, "-L", PKG_DIR, "-ldsqg_b200", "-Wl,-rpath,$ORIGIN", *link_ext])
     return LIB_PATH
 
 

@@ -395,7 +395,7 @@ static int decode_impl(const void* q, const void* k_new, const void* v_new,
                        void* k_ring, void* v_ring, const int32_t* head, const int32_t* fill,
                        const float* pos_bias, const float* scale_embed, const float* head_gain,
                        const int32_t* offsets, int J, int R,
-                       void* out, int S, int H, int D, int dtype, void* stream, bool overlap, bool interleaved = false) {
+                       void* out, int S, int H, int D, int dtype, void* stream, bool overlap, bool interleaved = false, uint8_t* kv_scale = nullptr) {
     if (!q || !k_new || !v_new || !k_ring || !v_ring || !head || !pos_bias || !out) return DSQG_ERR_NULL_POINTER;
     int rc = check_shape(S, H, 1, D, dtype);
     if (rc) return rc;
@@ -414,7 +414,7 @@ static int decode_impl(const void* q, const void* k_new, const void* v_new,
     a.scale = 1.0f / sqrtf((float)D);
     a.ring_stride = interleaved ? 2 * D : D;
     NvtxRange range(interleaved ? "dsqg_decode_kv" : "dsqg_decode");
-    cudaError_t e = launch_decode(a, t, dtype, static_cast<cudaStream_t>(stream), overlap);
+    cudaError_t e = kv_scale ? launch_decode8(a, kv_scale, t, dtype, static_cast<cudaStream_t>(stream), overlap) : launch_decode(a, t, dtype, static_cast<cudaStream_t>(stream), overlap);
     return e == cudaSuccess ? DSQG_OK : cuda_fail(e);
 }
 
@@ -455,6 +455,16 @@ int dsqg_decode_kv(const void* q, const void* k_new, const void* v_new, void* kv
     char* v_ring = static_cast<char*>(kv_ring) + (size_t)D * (dtype == DSQG_DTYPE_BF16 ? 2 : 4);
     return decode_impl(q, k_new, v_new, kv_ring, v_ring, head, fill, pos_bias, scale_embed, head_gain,
                        offsets, J, R, out, S, H, D, dtype, stream, overlapped != 0, true);
+}
+
+int dsqg_decode_kv_e4m3(const void* q, const void* k_new, const void* v_new, void* kv_ring, void* kv_scale, const int32_t* head, const int32_t* fill,
+                        const float* pos_bias, const float* scale_embed, const float* head_gain, const int32_t* offsets, int J, int R,
+                        void* out, int S, int H, int D, int dtype, void* stream, int overlapped) {
+    if (!kv_ring || !kv_scale) return DSQG_ERR_NULL_POINTER;
+    if (reinterpret_cast<uintptr_t>(kv_scale) & 1u) return DSQG_ERR_MISALIGNED;
+    // one ring of e4m3 rows: the value rows' pointer is not used
+    return decode_impl(q, k_new, v_new, kv_ring, kv_ring, head, fill, pos_bias, scale_embed, head_gain, offsets, J, R, out, S, H, D, dtype, stream,
+                       overlapped != 0, true, static_cast<uint8_t*>(kv_scale));
 }
 
 int dsqg_ring_advance(const int32_t* head, const int32_t* fill, int32_t* head_out, int32_t* fill_out, int S, int R, void* stream) {

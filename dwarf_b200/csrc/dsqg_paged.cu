@@ -1,0 +1,345 @@
+// The paged cache written from and read back to token-major tensors, and one new token's attention to it on CUDA cores, for every type and width.
+#include <cmath>
+
+#include "dsqg_paged.cuh"
+
+namespace dsqg {
+namespace {
+
+constexpr int kT = 256;
+
+// ---- prompts into pages and back.  Token t of a ragged batch belongs to the sequence s with cu[s] <= t < cu[s+1] and has position
+// start[s] + t - cu[s].  A group of lanes (8 elements a lane) takes the key and value rows of one (token, head) pair, so that the 2 D
+// elements of a cache slot are written together.  Bound by memory.
+struct MoveArgs {
+    PageArgs c;
+    const int32_t* cu; const int32_t* start;
+    void* k; void* v;
+    long long tokens, k_token, k_head, v_token, v_head;        // element strides
+    int dtype;
+};
+
+// (sequence, position) of token t, or s = -1: a row in front of the first sequence or behind the last.
+__device__ __forceinline__ int sequence_of(const MoveArgs& a, long long t, long long& position) {
+    int lo = 0, hi = a.c.S;
+    if (t < __ldg(a.cu) || t >= __ldg(a.cu + hi)) return -1;
+    while (hi - lo > 1) {                                       // cu[lo] <= t < cu[hi]
+        const int mid = (lo + hi) >> 1;
+        if (__ldg(a.cu + mid) <= t) lo = mid; else hi = mid;
+    }
+    position = t - __ldg(a.cu + lo) + (a.start ? __ldg(a.start + lo) : 0);
+    return lo;
+}
+
+template <int LPR, bool WRITE>
+__global__ void __launch_bounds__(kT) move_kernel(const MoveArgs a) {
+    stream_wait();
+    const long long pair = ((long long)blockIdx.x * kT + threadIdx.x) / LPR;
+    const int d = (threadIdx.x % LPR) * 8, D = a.c.D;
+    const long long t = pair / a.c.H;
+    const int h = (int)(pair - t * a.c.H);
+    const bool there = t < a.tokens, on = there && d < D;
+    long long position = 0, slot = -1;
+    int s = there ? sequence_of(a, t, position) : -1;
+    if (s >= 0 && position >= 0 && position < (long long)a.c.columns * a.c.page) {
+        const long long first = a.c.rows_of(s, h, (int)(position / a.c.page));
+        if (first >= 0) slot = (first + position % a.c.page) * 2;
+    }
+    const bool f8 = a.c.dtype == DSQG_DTYPE_E4M3;
+    const long long ki = t * a.k_token + h * a.k_head + d, vi = t * a.v_token + h * a.v_head + d;
+    float k[8] = {0, 0, 0, 0, 0, 0, 0, 0}, v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+    if constexpr (WRITE) {
+        if (on && slot >= 0) { load8_as(a.k, ki, a.dtype, k); load8_as(a.v, vi, a.dtype, v); }
+        if (f8) {
+            uint32_t kt = 0u, vt = 0u;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) { kt = max(kt, abs_bits(k[e])); vt = max(vt, abs_bits(v[e])); }
+            const uint32_t kb = row_scale_byte(group_max<LPR>(kt)), vb = row_scale_byte(group_max<LPR>(vt));
+            const float ik = scale_inverse(kb), iv = scale_inverse(vb);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) { k[e] *= ik; v[e] *= iv; }
+            if (d == 0 && slot >= 0) *reinterpret_cast<uint16_t*>(a.c.scale + slot) = (uint16_t)(kb | vb << 8);
+        }
+        if (on && slot >= 0) {
+            store8_as(a.c.kv, slot * D + d, a.c.dtype, k);
+            store8_as(a.c.kv, (slot + 1) * D + d, a.c.dtype, v);
+        }
+    } else if (on) {
+        if (slot >= 0) {
+            load8_as(a.c.kv, slot * D + d, a.c.dtype, k);
+            load8_as(a.c.kv, (slot + 1) * D + d, a.c.dtype, v);
+            if (f8) {
+                const uint32_t b = *reinterpret_cast<const uint16_t*>(a.c.scale + slot);
+                const float sk = scale_value(b & 255u), sv = scale_value(b >> 8);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) { k[e] *= sk; v[e] *= sv; }
+            }
+        } else if (s >= 0) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) k[e] = v[e] = __uint_as_float(0x7fc00000u);      // a position the table has no page for
+        }
+        store8_as(a.k, ki, a.dtype, k);
+        store8_as(a.v, vi, a.dtype, v);
+    }
+}
+
+template <bool WRITE> cudaError_t launch_move(const MoveArgs& a, cudaStream_t s) {
+    const int lanes = a.c.D / 8, lpr = lanes <= 1 ? 1 : lanes <= 2 ? 2 : lanes <= 4 ? 4 : lanes <= 8 ? 8 : 16;
+    const long long threads = a.tokens * a.c.H * lpr;
+    const unsigned blocks = (unsigned)((threads + kT - 1) / kT);
+    switch (lpr) {
+        case 1: return launch_after(move_kernel<1, WRITE>, blocks, kT, 0, s, a);
+        case 2: return launch_after(move_kernel<2, WRITE>, blocks, kT, 0, s, a);
+        case 4: return launch_after(move_kernel<4, WRITE>, blocks, kT, 0, s, a);
+        case 8: return launch_after(move_kernel<8, WRITE>, blocks, kT, 0, s, a);
+        default: return launch_after(move_kernel<16, WRITE>, blocks, kT, 0, s, a);
+    }
+}
+
+// ---- attention of one new token, CUDA cores: fp32 arithmetic for any types, D a multiple of 8 up to 128, pages of any length.
+// A block takes a part of one sequence for up to four query heads of one key-value head; a group of LPR lanes takes a position at a time and
+// keeps the running maximum and sum of its softmax for each of those heads; the groups are joined in shared memory in a fixed order.
+constexpr int kStepThreads = 128, kHeads = 4;
+
+template <int LPR>
+__global__ void __launch_bounds__(kStepThreads) step_kernel(const StepArgs a) {
+    __shared__ __align__(16) char fresh[2 * 128 * 4];
+    __shared__ uint8_t fresh_scale[2];
+    __shared__ float sm[kHeads][kStepThreads / LPR], sl[kHeads][kStepThreads / LPR];
+    __shared__ float sacc[kHeads][kStepThreads / LPR][LPR * 8];
+    stream_wait();
+    const PageArgs& c = a.c;
+    const int D = c.D, blocks_h = (a.G + kHeads - 1) / kHeads, hb = blockIdx.y % blocks_h, h = blockIdx.y / blocks_h, s = blockIdx.z, part = blockIdx.x;
+    const Range r = range_of(a, s, part);
+    if (part && r.first >= r.length) return;                   // part 0 always answers
+    const int heads = min(kHeads, a.G - hb * kHeads), q0 = (s * c.H + h) * a.G + hb * kHeads;
+    const int group = threadIdx.x / LPR, d = (threadIdx.x % LPR) * 8;
+    const bool on = d < D, has_new = a.k_new != nullptr && r.end == r.length && r.length > 0;
+    if (has_new) {
+        if (threadIdx.x < 32) new_row(a, s, h, r.length - 1, hb == 0, fresh, fresh_scale);
+        __syncthreads();
+    }
+    float q[kHeads][8], acc[kHeads][8], m[kHeads], l[kHeads];
+#pragma unroll
+    for (int i = 0; i < kHeads; ++i) {
+        m[i] = -INFINITY; l[i] = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) q[i][e] = acc[i][e] = 0.f;
+        if (on && i < heads) load8_as(a.q, (long long)(q0 + i) * D + d, a.q_f32 ? DSQG_DTYPE_F32 : DSQG_DTYPE_BF16, q[i]);
+    }
+    bool bad = r.bad;
+    const int last = has_new ? r.length - 1 : -1;
+    for (int p0 = r.first; p0 < r.end; p0 += kStepThreads / LPR) {
+        const int p = p0 + group;
+        float k[8] = {0, 0, 0, 0, 0, 0, 0, 0}, v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+        bool valid = p < r.end;
+        if (valid) {
+            const long long first = c.rows_of(s, h, p / c.page);
+            if (first < 0) { bad = true; valid = false; }
+            else if (on) {
+                const long long slot = (first + p % c.page) * 2;
+                const bool is_new = p == last;
+                const void* rows = is_new ? static_cast<const void*>(fresh) : c.kv;
+                load8_as(rows, is_new ? d : slot * D + d, c.dtype, k);
+                load8_as(rows, is_new ? D + d : (slot + 1) * D + d, c.dtype, v);
+                if (c.dtype == DSQG_DTYPE_E4M3) {
+                    const uint8_t* b = is_new ? fresh_scale : c.scale + slot;
+                    const float sk = scale_value(b[0]), sv = scale_value(b[1]);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) { k[e] *= sk; v[e] *= sv; }
+                }
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < kHeads; ++i) {
+            float dot = 0.f;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) dot = fmaf(q[i][e], k[e], dot);
+            dot = group_sum<LPR>(dot) * a.scale;
+            if (valid) {
+                const float mn = fmaxf(m[i], dot), base = mn == -INFINITY ? 0.f : mn;
+                const float cor = exp2f(m[i] - base), w = exp2f(dot - base);
+                l[i] = fmaf(l[i], cor, w);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) acc[i][e] = fmaf(acc[i][e], cor, w * v[e]);
+                m[i] = mn;
+            }
+        }
+    }
+    const bool any_bad = __syncthreads_or(bad);
+#pragma unroll
+    for (int i = 0; i < kHeads; ++i) {
+        if (d == 0) { sm[i][group] = m[i]; sl[i][group] = l[i]; }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sacc[i][group][d + e] = acc[i][e];
+    }
+    __syncthreads();
+    for (int o = threadIdx.x; o < heads * D; o += kStepThreads) {
+        const int i = o / D, e = o - i * D;
+        float M = -INFINITY;
+        for (int g = 0; g < kStepThreads / LPR; ++g) M = fmaxf(M, sm[i][g]);
+        const float base = M == -INFINITY ? 0.f : M;
+        float L = 0.f, A = 0.f;
+        for (int g = 0; g < kStepThreads / LPR; ++g) {
+            const float w = exp2f(sm[i][g] - base);
+            L = fmaf(w, sl[i][g], L); A = fmaf(w, sacc[i][g][e], A);
+        }
+        if (any_bad) L = A = __uint_as_float(0x7fc00000u);
+        if (a.ml) {
+            const long long at = (long long)(q0 + i) * a.parts + part;
+            if (e == 0) a.ml[at] = make_float2(M, L);
+            a.acc[at * D + e] = A;
+        } else {
+            const float y = L == 0.f ? 0.f : A / L;
+            const long long at = (long long)(q0 + i) * D + e;
+            if (a.q_f32) static_cast<float*>(a.out)[at] = y;
+            else static_cast<__nv_bfloat16*>(a.out)[at] = __float2bfloat16(y);
+        }
+    }
+}
+
+// Joins the parts of a sequence: one warp per (sequence, query head), parts in order.
+__global__ void __launch_bounds__(kT) join_kernel(const StepArgs a) {
+    stream_wait();
+    const int row = blockIdx.x * (kT / 32) + (threadIdx.x >> 5), lane = threadIdx.x & 31, D = a.c.D;
+    if (row >= a.c.S * a.c.H * a.G) return;
+    const int s = row / (a.c.H * a.G);
+    const Range r = range_of(a, s, 0);
+    const int n = r.length ? (r.length + a.chunk - 1) / a.chunk : 1;
+    const float2* ml = a.ml + (long long)row * a.parts;
+    float M = -INFINITY;
+    for (int p = lane; p < n; p += 32) M = fmaxf(M, ml[p].x);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+    const float base = M == -INFINITY ? 0.f : M;
+    float L = 0.f, A[4] = {0.f, 0.f, 0.f, 0.f};
+    const float* acc = a.acc + (long long)row * a.parts * D;
+    for (int p = 0; p < n; ++p) {
+        const float2 v = ml[p];
+        const float w = exp2f(v.x - base);
+        L = fmaf(w, v.y, L);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (lane + 32 * i < D) A[i] = fmaf(w, acc[(long long)p * D + lane + 32 * i], A[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int d = lane + 32 * i;
+        if (d >= D) break;
+        const float y = L == 0.f ? 0.f : A[i] / L;
+        if (a.q_f32) static_cast<float*>(a.out)[(long long)row * D + d] = y;
+        else static_cast<__nv_bfloat16*>(a.out)[(long long)row * D + d] = __float2bfloat16(y);
+    }
+}
+
+cudaError_t launch_step(const StepArgs& a, cudaStream_t s) {
+    const int lanes = a.c.D / 8;
+    const dim3 grid(a.parts, a.c.H * ((a.G + kHeads - 1) / kHeads), a.c.S);
+    if (lanes <= 1) return launch_after(step_kernel<1>, grid, kStepThreads, 0, s, a);
+    if (lanes <= 2) return launch_after(step_kernel<2>, grid, kStepThreads, 0, s, a);
+    if (lanes <= 4) return launch_after(step_kernel<4>, grid, kStepThreads, 0, s, a);
+    if (lanes <= 8) return launch_after(step_kernel<8>, grid, kStepThreads, 0, s, a);
+    return launch_after(step_kernel<16>, grid, kStepThreads, 0, s, a);
+}
+
+inline bool bad(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) != 0; }
+inline int status(cudaError_t e) { return e == cudaSuccess ? DSQG_OK : DSQG_ERR_CUDA; }
+
+// The positions of a part: a multiple of 64, from the sizes alone.
+struct Split { int chunk, parts; };
+inline Split split_for(int S, int H, int G, int limit) {
+    const long long pairs = (long long)S * H * ((G + 15) / 16);
+    const long long most = (limit + 63) / 64;                                  // in units of 64 positions
+    long long units = (pairs * most + 148 * 8 - 1) / (148 * 8);
+    if (units > 16) units = 16;
+    const long long least = (most + 1023) / 1024;                              // no more than 1024 parts
+    if (units < least) units = least;
+    if (units < 1) units = 1;
+    Split r;
+    r.chunk = (int)(units * 64);
+    r.parts = (int)((most + units - 1) / units);
+    if (r.parts < 1) r.parts = 1;
+    return r;
+}
+
+// A description of a cache that kernels may use.
+int page_args(const dsqg_pages* c, PageArgs* a) {
+    if (!c || !c->kv || !c->table || (c->dtype == DSQG_DTYPE_E4M3 && !c->scale)) return DSQG_ERR_NULL_POINTER;
+    if (c->dtype != DSQG_DTYPE_BF16 && c->dtype != DSQG_DTYPE_F32 && c->dtype != DSQG_DTYPE_E4M3) return DSQG_ERR_BAD_DTYPE;
+    if (c->sequences < 1 || c->sequences > 65535 || c->heads < 1 || c->heads > 65535 || c->pages < 1 || c->columns < 1 || c->page_size < 1 || c->D < 8 || c->D > 128 || c->D % 8 ||
+        (long long)c->columns * c->page_size > 0x7fffff00LL || (long long)c->pages * c->heads > 0x7fffffffffLL / ((long long)c->page_size * 2))
+        return DSQG_ERR_BAD_SHAPE;
+    if (bad(c->kv) || (reinterpret_cast<uintptr_t>(c->scale) & 1u)) return DSQG_ERR_MISALIGNED;
+    a->kv = static_cast<char*>(c->kv); a->scale = static_cast<uint8_t*>(c->scale); a->table = c->table;
+    a->dtype = c->dtype; a->pages = c->pages; a->page = c->page_size; a->columns = c->columns; a->H = c->heads; a->D = c->D; a->S = c->sequences;
+    a->row_bytes = c->D * (c->dtype == DSQG_DTYPE_F32 ? 4 : c->dtype == DSQG_DTYPE_BF16 ? 2 : 1);
+    return DSQG_OK;
+}
+
+int move_args(const dsqg_pages* c, const int32_t* cu, const int32_t* start, void* k, void* v, long long k_token, long long k_head, long long v_token, long long v_head,
+              long long tokens, int dtype, MoveArgs* a) {
+    if (!cu || !k || !v) return DSQG_ERR_NULL_POINTER;
+    if (int rc = page_args(c, &a->c)) return rc;
+    if (dtype != DSQG_DTYPE_BF16 && dtype != DSQG_DTYPE_F32) return DSQG_ERR_BAD_DTYPE;
+    if (tokens < 1 || tokens > 0x7fffffffLL || tokens * c->heads * 16 > 0x7fffffffLL * kT) return DSQG_ERR_BAD_SHAPE;
+    if (bad(k) || bad(v) || k_token % 8 || k_head % 8 || v_token % 8 || v_head % 8) return DSQG_ERR_MISALIGNED;
+    a->cu = cu; a->start = start; a->k = k; a->v = v; a->tokens = tokens; a->dtype = dtype;
+    a->k_token = k_token; a->k_head = k_head; a->v_token = v_token; a->v_head = v_head;
+    return DSQG_OK;
+}
+
+}  // namespace
+}  // namespace dsqg
+
+using namespace dsqg;
+
+extern "C" {
+
+int dsqg_paged_write(const dsqg_pages* cache, const void* k, const void* v, long long k_token, long long k_head, long long v_token, long long v_head,
+                     const int32_t* cu_seqlens, const int32_t* start, long long tokens, int dtype, void* stream) {
+    MoveArgs a;
+    if (int rc = move_args(cache, cu_seqlens, start, const_cast<void*>(k), const_cast<void*>(v), k_token, k_head, v_token, v_head, tokens, dtype, &a)) return rc;
+    return status(launch_move<true>(a, static_cast<cudaStream_t>(stream)));
+}
+
+int dsqg_paged_read(const dsqg_pages* cache, void* k, void* v, const int32_t* cu_seqlens, const int32_t* start, long long tokens, int dtype, void* stream) {
+    MoveArgs a;
+    const long long D = cache ? cache->D : 0, HD = cache ? D * cache->heads : 0;
+    if (int rc = move_args(cache, cu_seqlens, start, k, v, HD, D, HD, D, tokens, dtype, &a)) return rc;
+    return status(launch_move<false>(a, static_cast<cudaStream_t>(stream)));
+}
+
+size_t dsqg_paged_step_scratch_bytes(int sequences, int heads, int q_heads, int D, int max_length) {
+    if (sequences < 1 || heads < 1 || q_heads < heads || q_heads % heads || D < 1 || max_length < 0) return 0;
+    const Split p = split_for(sequences, heads, q_heads / heads, max_length);
+    return p.parts == 1 ? 0 : (size_t)sequences * q_heads * p.parts * (D + 2) * 4;
+}
+
+int dsqg_paged_step(const dsqg_pages* cache, const void* q, const void* k_new, const void* v_new, const int32_t* lengths, int q_heads, int max_length, float scale,
+                    void* out, void* scratch, size_t scratch_bytes, int dtype, void* stream) {
+    StepArgs a;
+    if (!q || !lengths || !out || !k_new != !v_new) return DSQG_ERR_NULL_POINTER;
+    if (int rc = page_args(cache, &a.c)) return rc;
+    if (dtype != DSQG_DTYPE_BF16 && dtype != DSQG_DTYPE_F32) return DSQG_ERR_BAD_DTYPE;
+    if (q_heads < a.c.H || q_heads % a.c.H || (long long)a.c.S * q_heads > 0x7fffffffLL / 128 || max_length < 0 || a.c.H * ((q_heads / a.c.H + 3) / 4) > 65535) return DSQG_ERR_BAD_SHAPE;
+    if (!(scale < 3.0e38f)) return DSQG_ERR_UNSUPPORTED;
+    if (bad(q) || bad(k_new) || bad(v_new) || bad(out) || bad(scratch)) return DSQG_ERR_MISALIGNED;
+    if (max_length > (long long)a.c.columns * a.c.page) return DSQG_ERR_BAD_SHAPE;
+    a.limit = max_length;
+    a.q = q; a.k_new = k_new; a.v_new = v_new; a.lengths = lengths; a.out = out; a.G = q_heads / a.c.H; a.q_f32 = dtype == DSQG_DTYPE_F32;
+    a.scale = (scale > 0.f ? scale : 1.0f / sqrtf((float)a.c.D)) * 1.4426950408889634f;
+    const Split p = split_for(a.c.S, a.c.H, a.G, a.limit);
+    a.chunk = p.chunk; a.parts = p.parts; a.ml = nullptr; a.acc = nullptr;
+    if (p.parts > 1) {
+        const size_t rows = (size_t)a.c.S * q_heads * p.parts;
+        if (!scratch) return DSQG_ERR_NULL_POINTER;
+        if (scratch_bytes < rows * (a.c.D + 2) * 4) return DSQG_ERR_SCRATCH_TOO_SMALL;
+        a.ml = static_cast<float2*>(scratch); a.acc = static_cast<float*>(scratch) + 2 * rows;
+    }
+    const cudaStream_t s = static_cast<cudaStream_t>(stream);
+    cudaError_t e = paged_mma_supported(a) ? launch_paged_mma(a, s) : launch_step(a, s);
+    if (e == cudaSuccess && a.ml) e = launch_after(join_kernel, (a.c.S * q_heads + kT / 32 - 1) / (kT / 32), kT, 0, s, a);
+    return status(e);
+}
+
+}  // extern "C"

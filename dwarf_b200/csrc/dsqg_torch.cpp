@@ -4,14 +4,7 @@
 // kernels of small problems and of a decode step take.
 //
 // PyTorch supplies device memory, streams and the autograd graph only; all arithmetic is in libdsqg_b200.so.
-#include <torch/extension.h>
-
-#include <ATen/autocast_mode.h>
-#include <ATen/cuda/CUDAContext.h>
-#include <ATen/cuda/EmptyTensor.h>
-#include <c10/cuda/CUDACachingAllocator.h>
-#include <c10/cuda/CUDAGuard.h>
-#include <torch/csrc/Exceptions.h>
+#include "dsqg_torch.h"
 
 #include <cublasLt.h>
 #include <cublas_v2.h>
@@ -21,24 +14,8 @@
 #include <map>
 #include <memory>
 #include <mutex>
-#include <optional>
-#include <sstream>
-
-#include "dsqg_b200.h"
-
-namespace py = pybind11;
-using at::Tensor;
-using torch::autograd::AutogradContext;
-using torch::autograd::variable_list;
 
 namespace {
-
-// An offset set, converted once and kept for the life of the process (programs use a handful): autograd nodes and
-// the Python cache (ops._offsets) hold plain pointers to it.
-struct Offsets {
-    std::vector<int32_t> v;
-    int J() const { return (int)v.size(); }
-};
 
 const Offsets* intern_offsets(const std::vector<int32_t>& v) {
     static std::mutex mu;
@@ -47,77 +24,6 @@ const Offsets* intern_offsets(const std::vector<int32_t>& v) {
     std::unique_ptr<Offsets>& o = table[v];
     if (!o) { o = std::make_unique<Offsets>(); o->v = v; }
     return o.get();
-}
-
-// Raises dwarf_b200.DSQGError for a non-zero status.
-void check(int status, const char* where) {
-    if (status == DSQG_OK) return;
-    py::gil_scoped_acquire gil;
-    py::module_::import("dwarf_b200._lib").attr("check")(status, where);
-    throw std::runtime_error(std::string(where) + " failed");
-}
-
-// Runs the body of a backward node: the autograd engine's threads carry Python errors in its own exception type, and start
-// without a CUDA context, which cuBLAS would remark on.
-template <typename F> auto backward_body(const Tensor& on, F f) {
-    static thread_local int ready = -1;
-    if (on.defined() && on.is_cuda() && ready != on.device().index()) {
-        ready = on.device().index();
-        const int before = c10::cuda::current_device();
-        c10::cuda::SetDevice(ready, /*force=*/true);
-        c10::cuda::SetDevice(before);
-    }
-    try {
-        return f();
-    } catch (py::error_already_set& e) {
-        py::gil_scoped_acquire gil;
-        e.restore();
-        python_error err;
-        err.persist();
-        throw err;
-    }
-}
-
-int dtype_code(const Tensor& t) {
-    if (t.scalar_type() == at::kBFloat16) return DSQG_DTYPE_BF16;
-    if (t.scalar_type() == at::kFloat) return DSQG_DTYPE_F32;
-    throw py::type_error(std::string("dsqg: q/k/v must be bfloat16 or float32, got ") + toString(t.scalar_type()));
-}
-
-std::string shape_of(const Tensor& t) {
-    std::ostringstream s;
-    s << t.sizes();
-    return s.str();
-}
-
-void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
-float* fptr(const Tensor& t) { return t.defined() ? static_cast<float*>(t.data_ptr()) : nullptr; }
-void* stream_of(const Tensor& t) { return at::cuda::getCurrentCUDAStream(t.device().index()).stream(); }
-
-// Uninitialised device tensors straight from the allocator: a dispatched at::empty costs 2.6 us on an autograd thread, this
-// one less than a third, and a backward call makes six.
-Tensor new_tensor(at::IntArrayRef sizes, at::ScalarType dt, const Tensor& on) { return at::detail::empty_cuda(sizes, dt, on.device(), std::nullopt); }
-Tensor new_like(const Tensor& t) { return t.defined() ? new_tensor(t.sizes(), t.scalar_type(), t) : t; }
-
-// A parameter as the kernels read it: fp32 and contiguous (no copy where it is so already; it may be the caller's own tensor).
-Tensor f32c(const Tensor& t) {
-    if (!t.defined() || (t.scalar_type() == at::kFloat && t.is_contiguous())) return t;
-    return t.detach().to(at::kFloat).contiguous();
-}
-// The kernels around the GEMMs and the GEMM plans want 16-byte pointers; a parameter that is a view of a flat buffer, or a caller's
-// activation, may start anywhere and is copied then.
-bool on_16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
-Tensor aligned(const Tensor& t) { return !t.defined() || on_16(t.data_ptr()) ? t : t.detach().clone(); }
-Tensor like_param(Tensor g, at::ScalarType dt) { return g.defined() && g.scalar_type() != dt ? g.to(dt) : g; }
-Tensor opt(const std::optional<Tensor>& t) { return t.has_value() ? *t : Tensor(); }
-at::ScalarType type_of(const Tensor& t) { return t.defined() ? t.scalar_type() : at::kFloat; }
-
-bool shape_is(const Tensor& t, std::initializer_list<int64_t> s) { return t.sizes() == at::IntArrayRef(s); }
-
-// The kernels get plain pointers: a tensor on the host or on another GPU would be read as if it were on this one.
-void check_device(const char* who, const Tensor& on, std::initializer_list<const Tensor*> ts) {
-    for (const Tensor* t : ts)
-        if (t->defined() && t->device() != on.device()) throw py::value_error(std::string(who) + ": all tensors must be on " + on.device().str() + ", got one on " + t->device().str());
 }
 
 void check_inputs(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& pb, const Tensor& hg, const Tensor& se, int J) {
@@ -151,9 +57,6 @@ int64_t padded_head_dim(int64_t D, bool bf16, const Offsets& off, bool has_se) {
 }
 
 Tensor pad_to(const Tensor& t, int64_t Dp) { return t.defined() ? at::constant_pad_nd(t, {0, Dp - t.size(-1)}) : t; }
-
-// Scratch for one backward call, returned to the caching allocator when it leaves scope.
-at::DataPtr scratch_for(size_t bytes) { return c10::cuda::CUDACachingAllocator::get()->allocate(bytes); }
 
 // ------------------------------------------------------------------------------------ dsqg_attention
 struct Forward { Tensor q, k, v, pb, hg, se, out, lse; int64_t D; };
@@ -225,13 +128,6 @@ struct AttentionNode : torch::autograd::Function<AttentionNode> {
                 like_param(dhg, type_at(ctx, 1)), like_param(narrow_cols(dse, D), type_at(ctx, 2)), Tensor()};
     }
 };
-
-bool wants_grad(std::initializer_list<const Tensor*> ts) {
-    if (!at::GradMode::is_enabled()) return false;
-    for (const Tensor* t : ts)
-        if (t->defined() && t->requires_grad()) return true;
-    return false;
-}
 
 Tensor attention(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& pb, const std::optional<Tensor>& hg,
                  const std::optional<Tensor>& se, const Offsets* off) {
@@ -824,18 +720,31 @@ Tensor decode_step(const Tensor& q, const Tensor& k, const Tensor& v, const Tens
 // kv_ring [S,H,R,2,D], or the rings of all layers [L,S,H,R,2,D] and the layer to use
 Tensor decode_step_kv(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& kv, std::optional<int64_t> layer0, const Tensor& head, const Tensor& pos_bias,
                       const std::optional<Tensor>& hg, const std::optional<Tensor>& se, const Offsets* off,
-                      const std::optional<Tensor>& fill0, const std::optional<Tensor>& out0, bool overlap) {
+                      const std::optional<Tensor>& fill0, const std::optional<Tensor>& out0, bool overlap, const std::optional<Tensor>& kv_scale) {
     const int64_t lead = layer0.has_value() ? 1 : 0;
     if (kv.dim() != 5 + lead || kv.size(3 + lead) != 2 || !kv.is_contiguous()) throw py::value_error("dsqg_decode_kv: kv_ring must be contiguous [S,H,R,2,D]");
     const int64_t layer = !lead ? 0 : *layer0 < 0 ? *layer0 + kv.size(0) : *layer0;
     if (lead && (layer < 0 || layer >= kv.size(0))) throw py::index_error("dsqg_decode_kv: no such layer");
     const int64_t S = kv.size(lead), H = kv.size(1 + lead), R = kv.size(2 + lead), D = kv.size(4 + lead);
     const Tensor fill = opt(fill0);
-    check_step("dsqg_decode_kv", q, k, v, kv.scalar_type(), S, H, D, kv, head, fill, pos_bias, opt(hg), opt(se), off->J());
+    const bool f8 = kv.scalar_type() == at::kFloat8_e4m3fn;
+    if (f8 != kv_scale.has_value()) throw py::value_error("dsqg_decode_kv: kv_scale belongs to a ring in float8_e4m3fn");
+    if (f8 && ((kv_scale->scalar_type() != at::kFloat8_e8m0fnu && kv_scale->scalar_type() != at::kByte) || !kv_scale->is_contiguous() ||
+               kv_scale->sizes() != kv.sizes().slice(0, 4 + lead)))
+        throw py::value_error("dsqg_decode_kv: kv_scale must be contiguous [S,H,R,2] float8_e8m0fnu");
+    if (f8) dtype_code(q);
+    check_step("dsqg_decode_kv", q, k, v, f8 ? q.scalar_type() : kv.scalar_type(), S, H, D, kv, head, fill, pos_bias, opt(hg), opt(se), off->J());
+    if (f8) check_device("dsqg_decode_kv", q, {&*kv_scale});
     const StepParams p = {f32c(pos_bias), f32c(opt(hg)), f32c(opt(se))};
     const c10::cuda::CUDAGuard guard(q.device());
     Tensor out = out0.has_value() ? *out0 : new_like(q);
     char* ring = static_cast<char*>(kv.data_ptr()) + (lead ? layer * kv.stride(0) * kv.element_size() : 0);
+    if (f8) {
+        char* scale = static_cast<char*>(kv_scale->data_ptr()) + (lead ? layer * kv_scale->stride(0) : 0);
+        check(dsqg_decode_kv_e4m3(ptr(q), ptr(k), ptr(v), ring, scale, static_cast<const int32_t*>(ptr(head)), static_cast<const int32_t*>(ptr(fill)), fptr(p.pb), fptr(p.se),
+                                  fptr(p.hg), off->v.data(), off->J(), (int)R, ptr(out), (int)S, (int)H, (int)D, dtype_code(q), stream_of(q), overlap), "dsqg_decode_kv_e4m3");
+        return out;
+    }
     check(dsqg_decode_kv(ptr(q), ptr(k), ptr(v), ring, static_cast<const int32_t*>(ptr(head)), static_cast<const int32_t*>(ptr(fill)),
                          fptr(p.pb), fptr(p.se), fptr(p.hg), off->v.data(), off->J(), (int)R, ptr(out), (int)S, (int)H, (int)D, dtype_code(q),
                          stream_of(q), overlap), "dsqg_decode_kv");
@@ -869,4 +778,5 @@ PYBIND11_MODULE(_dsqg_torch, m) {
     m.def("decode_step", &decode_step);
     m.def("decode_step_kv", &decode_step_kv);
     m.def("ring_advance", &ring_advance);
+    bind_serving(m);
 }

@@ -55,6 +55,23 @@ def causal_mean(x):
     return _lib.native().causal_mean(x.float()).to(x.dtype)
 
 
+def rms_norm(x, weight, residual=None, eps=1e-6, out_dtype=None):
+    """Root-mean-square norm, the residual's addition in front of it included: h = x + residual in residual's type, y = h / sqrt(mean(h^2) + eps) *
+    weight over the last dimension.  x, residual bf16 or fp32 [..., D], each its own type (a bf16 branch onto an fp32 stream); weight [D];
+    out_dtype: bf16 or fp32, default that of the stream.  Returns y, or (y, h) with a residual.  One pass over memory; differentiable in all
+    three tensors (the pre-norm blocks of the benchmark model, `x = x + f(x); norm(x)`)."""
+    y, h = _lib.native().rms_norm(x, weight, residual, eps, out_dtype)
+    return y if residual is None else (y, h)
+
+
+def rms_norm_e4m3(x, weight, residual=None, eps=1e-6):
+    """rms_norm with its output in 8 bits: (y float8_e4m3fn [..., D], scale float8_e8m0fnu [...]) and, with a residual, h.  A row's scale is the
+    smallest power of two 2^e, e >= -126, with max|row| <= 448 * 2^e (1 for a row of zeros; NaN where the row has a NaN or an infinity).  No
+    backward pass."""
+    y, scale, h = _lib.native().rms_norm_e4m3(x, weight, residual, eps)
+    return (y, scale) if residual is None else (y, scale, h)
+
+
 class DSQGPackedFunction:
     """DSQG on the un-permuted output of a fused qkv projection, with a token-major result (an autograd node in
     native code, csrc/dsqg_torch.cpp).

@@ -52,7 +52,7 @@ typedef enum {
     DSQG_ERR_WAIT = -10           /* dsqg_weight_grads: a wait in an earlier call on this device gave up (see dsqg_device_error) */
 } dsqg_status;
 
-enum { DSQG_DTYPE_BF16 = 0, DSQG_DTYPE_F32 = 1 };
+enum { DSQG_DTYPE_BF16 = 0, DSQG_DTYPE_F32 = 1, DSQG_DTYPE_E4M3 = 2 /* where an entry says so */ };
 
 /* Human-readable text for a status code.  Never NULL. */
 const char* dsqg_status_str(int status);
@@ -393,6 +393,71 @@ int dsqg_decode_overlapped(const void* q, const void* k_new, const void* v_new,
  * (capped at R), which is what dsqg_decode expects. */
 int dsqg_ring_prefill(const void* k, const void* v, void* k_ring, void* v_ring,
                       int32_t* head, int32_t* fill, int S, int H, int N, int D, int R, int dtype, void* stream);
+
+/* ---- Serving in fewer bits: norms, caches, one new token's attention, projections ---------------------------------------
+ * No counterpart in the reference, whose generate() re-runs the whole prefix in the training types (DWARF
+ * train/train_2048_condU.py:463-487).
+ * Rows in 8 bits: e4m3 values and one scale byte per row, a power of two 2^(byte - 127) (255: NaN): the smallest 2^e, e >= -126, with
+ * max|row| <= 448 2^e, and 1 for a row of zeros.  A row with a NaN or an infinity in it is NaN as a whole.  All pointers are DEVICE pointers, 16-byte
+ * aligned where they point at elements of rows; scale bytes of keys and values on 2 bytes. */
+
+/* Root-mean-square norm of a residual stream, the addition in front of it included:
+ *     h = x + residual (rounded to stream_dtype), y = h / sqrt(mean(h^2) + eps) * weight.
+ * x, residual: bf16 or fp32 [rows,D], each its own type; residual nullable: h = x, which is not written.  y: bf16, fp32 or e4m3 with y_scale
+ * [rows].  rstd [rows] fp32 (nullable): 1 / sqrt(..), for the backward pass.  Any D >= 1; rows start on 16 bytes and are read in pieces of eight
+ * elements where D is a multiple of 8.  h may be residual or x where the types allow it. */
+typedef struct dsqg_rms_norm {
+    const void* x; const void* residual; const float* weight;
+    void* h; void* y; void* y_scale; float* rstd;
+    long long rows; int D; float eps;
+    int x_dtype, stream_dtype, y_dtype;
+} dsqg_rms_norm;
+int dsqg_rms_norm_fwd(const dsqg_rms_norm* p, void* stream);
+/* Its backward pass for the gradients dy (y_dtype: bf16 or fp32) and dh (nullable, like h) of y and h:
+ *     d = dh + rstd (w dy - x^ mean(w dy x^)), x^ = h rstd;  dx = d (x_dtype), dresidual = d (stream_dtype), dweight = sum over rows of dy x^.
+ * Any of the three may be NULL.  Reads weight, rstd and h (x without a residual) of p.  The order of the sums follows from rows and D alone. */
+size_t dsqg_rms_norm_bwd_scratch_bytes(long long rows, int D);
+int dsqg_rms_norm_bwd(const dsqg_rms_norm* p, const void* dy, const void* dh, void* dx, void* dresidual, float* dweight, void* scratch, size_t scratch_bytes, void* stream);
+
+/* dsqg_decode_kv and dsqg_ring_prefill_kv over a ring in 8 bits: kv_ring e4m3 [S,H,R,2,D], kv_scale [S,H,R,2] bytes.  dtype: of q, k_new, v_new
+ * and out (k, v of the prefill), bf16 or fp32.  The step attends to what the ring holds, the new token's quantised rows included. */
+int dsqg_decode_kv_e4m3(const void* q, const void* k_new, const void* v_new, void* kv_ring, void* kv_scale, const int32_t* head, const int32_t* fill,
+                        const float* pos_bias, const float* scale_embed, const float* head_gain, const int32_t* offsets, int J, int R,
+                        void* out, int S, int H, int D, int dtype, void* stream, int overlapped);
+int dsqg_ring_prefill_e4m3(const void* k, const void* v, void* kv_ring, void* kv_scale, int32_t* head, int32_t* fill, int S, int H, int N, int D, int R, int dtype,
+                           void* stream);
+/* out [rows,D] (bf16 or fp32) = the values of x [rows,D] e4m3 with scale [rows] bytes; D a multiple of 8. */
+int dsqg_dequantize_rows(const void* x, const void* scale, void* out, long long rows, int D, int dtype, void* stream);
+
+/* A paged key-value cache of one layer.  kv [pages,heads,page_size,2,D] in bf16, fp32 or e4m3 (then scale [pages,heads,page_size,2] bytes): a page holds
+ * page_size consecutive positions of one sequence, key and value of a position side by side.  table int32 [sequences,columns]: the page of positions
+ * [c page_size, (c+1) page_size) of a sequence.  An entry that is no index of a page is never followed: what would be written there is dropped, what
+ * would be read is NaN. */
+typedef struct dsqg_pages {
+    void* kv; void* scale; const int32_t* table;
+    int dtype, sequences, columns, pages, page_size, heads, D;
+} dsqg_pages;
+/* The keys and values of a ragged batch into their pages, and back.  Token t of the batch belongs to the sequence s with
+ * cu_seqlens[s] <= t < cu_seqlens[s+1] (int32 [sequences+1], ascending) and has position start[s] + t - cu_seqlens[s] (start nullable: 0).  k, v: bf16 or
+ * fp32, D contiguous elements per token and head; the write takes element strides (multiples of 8), the read fills [tokens,heads,D].  Tokens of no
+ * sequence are not written; read, they are zeros.  */
+int dsqg_paged_write(const dsqg_pages* cache, const void* k, const void* v, long long k_token, long long k_head, long long v_token, long long v_head,
+                     const int32_t* cu_seqlens, const int32_t* start, long long tokens, int dtype, void* stream);
+int dsqg_paged_read(const dsqg_pages* cache, void* k, void* v, const int32_t* cu_seqlens, const int32_t* start, long long tokens, int dtype, void* stream);
+/* One new token per sequence: out[s,i] = softmax(scale q[s,i] . K^T) V over the lengths[s] positions of sequence s, for query heads i of key-value head
+ * i / (q_heads / heads).  q, out [sequences,q_heads,D], k_new, v_new [sequences,heads,D] in dtype (bf16 or fp32).  With k_new, v_new (both or
+ * neither) the token at position lengths[s] - 1 is stored first and attended to as stored.  lengths int32 [sequences], 0 <= lengths[s] <= max_length <=
+ * columns * page_size: 0 gives zeros and stores nothing, a length outside gives NaN.  Long sequences are split and joined (scratch; the order of the
+ * sums follows from the sizes, max_length among them, and from the sequence's own length).  scale <= 0: 1/sqrt(D). */
+size_t dsqg_paged_step_scratch_bytes(int sequences, int heads, int q_heads, int D, int max_length);
+int dsqg_paged_step(const dsqg_pages* cache, const void* q, const void* k_new, const void* v_new, const int32_t* lengths, int q_heads, int max_length, float scale,
+                    void* out, void* scratch, size_t scratch_bytes, int dtype, void* stream);
+
+/* y [M,N] bf16 = x [M,K] W^T + bias, W[n,k] = (nibble - 8) * scales[n, k / group]: weight [N,K/2] bytes, the nibble of an even k in the low half;
+ * scales bf16 [N,K/group], group 32, 64 or 128, K a multiple of it; bias fp32 [N], nullable.  x: bf16, or e4m3 with x_scale [M] bytes.  fp32 sums; made
+ * for a few rows (a decode step): 16 rows at a time read the weights once. */
+int dsqg_int4_linear(const void* x, const void* x_scale, const void* weight, const void* scales, const float* bias, void* y, int M, int N, int K, int group, int dtype,
+                     void* stream);
 
 #ifdef __cplusplus
 }
