@@ -198,37 +198,50 @@ __global__ void __launch_bounds__(kStepThreads) step_kernel(const StepArgs a) {
     }
 }
 
-// Joins the parts of a sequence: one warp per (sequence, query head), parts in order.
-__global__ void __launch_bounds__(kT) join_kernel(const StepArgs a) {
+// Joins the parts of a sequence: one block per (sequence, query head), its warps every eighth part, added in warp order.  (One warp per row, parts one
+// after the other: 40 us for 128 rows of 98 parts, which is a chain of loads.)
+constexpr int kJoinWarps = 8;
+__global__ void __launch_bounds__(kJoinWarps * 32) join_kernel(const StepArgs a) {
+    __shared__ float4 sums[kJoinWarps][32];
+    __shared__ float sl[kJoinWarps];
     stream_wait();
-    const int row = blockIdx.x * (kT / 32) + (threadIdx.x >> 5), lane = threadIdx.x & 31, D = a.c.D;
-    if (row >= a.c.S * a.c.H * a.G) return;
+    const int row = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, D = a.c.D, d = 4 * lane;
     const int s = row / (a.c.H * a.G);
     const Range r = range_of(a, s, 0);
     const int n = r.length ? (r.length + a.chunk - 1) / a.chunk : 1;
     const float2* ml = a.ml + (long long)row * a.parts;
+    const float* acc = a.acc + (long long)row * a.parts * D;
     float M = -INFINITY;
     for (int p = lane; p < n; p += 32) M = fmaxf(M, ml[p].x);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
     const float base = M == -INFINITY ? 0.f : M;
-    float L = 0.f, A[4] = {0.f, 0.f, 0.f, 0.f};
-    const float* acc = a.acc + (long long)row * a.parts * D;
-    for (int p = 0; p < n; ++p) {
+    float L = 0.f;
+    float4 A = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int p = warp; p < n; p += kJoinWarps) {
         const float2 v = ml[p];
+        const float4 x = d < D ? *reinterpret_cast<const float4*>(acc + (long long)p * D + d) : A;
         const float w = exp2f(v.x - base);
         L = fmaf(w, v.y, L);
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (lane + 32 * i < D) A[i] = fmaf(w, acc[(long long)p * D + lane + 32 * i], A[i]);
+        A.x = fmaf(w, x.x, A.x); A.y = fmaf(w, x.y, A.y); A.z = fmaf(w, x.z, A.z); A.w = fmaf(w, x.w, A.w);
     }
+    sums[warp][lane] = A;
+    if (lane == 0) sl[warp] = L;
+    __syncthreads();
+    if (warp || d >= D) return;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int d = lane + 32 * i;
-        if (d >= D) break;
-        const float y = L == 0.f ? 0.f : A[i] / L;
-        if (a.q_f32) static_cast<float*>(a.out)[(long long)row * D + d] = y;
-        else static_cast<__nv_bfloat16*>(a.out)[(long long)row * D + d] = __float2bfloat16(y);
+    for (int w = 1; w < kJoinWarps; ++w) {
+        const float4 x = sums[w][lane];
+        A.x += x.x; A.y += x.y; A.z += x.z; A.w += x.w;
+        L += sl[w];
+    }
+    const float y[4] = {A.x, A.y, A.z, A.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const float z = L == 0.f ? 0.f : y[e] / L;
+        if (a.q_f32) static_cast<float*>(a.out)[(long long)row * D + d + e] = z;
+        else static_cast<__nv_bfloat16*>(a.out)[(long long)row * D + d + e] = __float2bfloat16(z);
     }
 }
 
@@ -250,8 +263,8 @@ struct Split { int chunk, parts; };
 inline Split split_for(int S, int H, int G, int limit) {
     const long long pairs = (long long)S * H * ((G + 15) / 16);
     const long long most = (limit + 63) / 64;                                  // in units of 64 positions
-    long long units = (pairs * most + 148 * 8 - 1) / (148 * 8);
-    if (units > 16) units = 16;
+    long long units = (pairs * most + 148 * 4 - 1) / (148 * 4);                // as many blocks as run at once ...
+    if (units > 32) units = 32;                                                // ... of up to 2048 positions: sequences differ in length
     const long long least = (most + 1023) / 1024;                              // no more than 1024 parts
     if (units < least) units = least;
     if (units < 1) units = 1;
@@ -334,11 +347,11 @@ int dsqg_paged_step(const dsqg_pages* cache, const void* q, const void* k_new, c
         const size_t rows = (size_t)a.c.S * q_heads * p.parts;
         if (!scratch) return DSQG_ERR_NULL_POINTER;
         if (scratch_bytes < rows * (a.c.D + 2) * 4) return DSQG_ERR_SCRATCH_TOO_SMALL;
-        a.ml = static_cast<float2*>(scratch); a.acc = static_cast<float*>(scratch) + 2 * rows;
+        a.acc = static_cast<float*>(scratch); a.ml = reinterpret_cast<float2*>(a.acc + rows * a.c.D);
     }
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     cudaError_t e = paged_mma_supported(a) ? launch_paged_mma(a, s) : launch_step(a, s);
-    if (e == cudaSuccess && a.ml) e = launch_after(join_kernel, (a.c.S * q_heads + kT / 32 - 1) / (kT / 32), kT, 0, s, a);
+    if (e == cudaSuccess && a.ml) e = launch_after(join_kernel, a.c.S * q_heads, kJoinWarps * 32, 0, s, a);
     return status(e);
 }
 

@@ -1,14 +1,20 @@
 // One new token's attention to a paged cache on tensor cores: bf16 queries, pages in bf16 or e4m3, D = 32, 64, 96 or 128.
 //
-// A block takes a part of one sequence for up to 16 query heads of one key-value head, a warp every fourth tile of 16 positions of it.  The query
-// heads are the 16 rows of mma.sync (m16n8k16, fp32 accumulators): S = Q K^T, softmax with a running maximum and sum per row, O += P V.  The
-// contraction of a product may be permuted freely as long as both operands agree, so every lane reads exactly the 16-byte pieces of a tile that it
-// needs itself: it copies them into shared memory with cp.async some tiles ahead and reads back its own bytes, with no barrier and no bank
-// conflict, and no register is held by a load in flight.  Key rows are the B operand as they lie (lane (g, t): row g, every fourth piece from t);
-// of the value rows a lane takes four positions and an eighth of the columns, and pairs of positions are put together by byte permutation.
+// A block takes a part of one sequence for up to 8 HT query heads of one key-value head, a warp every fourth tile of 16 positions of it.  Positions are
+// the 16 rows of mma.sync (m16n8k16, fp32 accumulators) and the query heads its 8 columns: S^T = K Q^T, softmax with a running maximum and sum per
+// column, O^T += V^T P^T.  A tile is one run of memory (a page keeps key and value of a position side by side): a warp copies its tiles to shared memory
+// with cp.async, some rounds ahead, 512 consecutive bytes an instruction, and waits for nobody but itself.  (Every lane copying the pieces that
+// it needs itself, 64 to 128 bytes a row: 68 us of copies alone for 4 sequences of 100001 positions, 4 x 8 heads of 128 in 8 bits, against 51.)  The
+// 16-byte pieces of a row are exchanged by s(row), so that the reads below are free of bank conflicts.  The contraction of a product, and the rows of
+// its result, may be permuted freely: key rows are the A operand as they lie (lane (g, t): rows g and g + 8, every fourth piece from t); of the value
+// rows a lane takes four positions and an eighth of the columns, and pairs of positions are put together by byte permutation.
+// P^T turns from a result into an operand by movmatrix.
 //
 // 8 bits: e4m3 becomes f16 exactly.  Queries become f16 after a power of two that brings their largest element near 1; the keys' scales multiply the
 // scores; the values' scales multiply the probabilities, relative to the largest scale seen so far (another running maximum), so that f16 holds them.
+//
+// (Query heads as the 16 rows of the product instead: half of every accumulator idle up to 8 heads, 179 registers, 8 warps an SM and 636 instructions a
+// tile of 8-bit rows of 128 columns; 160 us for 4 sequences of 100001 positions, 4 x 8 heads.)
 //
 // mma.sync and not tcgen05: an operand of 128 rows would be at most an eighth full (query heads of one key-value head), and what is in question is memory.
 #include "dsqg_paged.cuh"
@@ -17,6 +23,10 @@ namespace dsqg {
 namespace {
 
 constexpr int kWarps = 4, kTile = 16;
+// A new maximum rescales what was summed so far only if it is above the old one by more than this (in powers of two): probabilities stay below 2^8, which
+// f16, bf16 and the fp32 sums hold as well as those below 1.  A warp then rescales once or twice; at every new maximum of any of eight heads it did so at
+// 13 of its first 16 tiles.
+constexpr float kSlack = 8.f;
 
 template <bool F16> __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     if constexpr (F16)
@@ -27,131 +37,151 @@ template <bool F16> __device__ __forceinline__ void mma(float (&c)[4], const uin
             : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 // BYTES from global to shared memory, zeros where `on` is false.
-template <int BYTES> __device__ __forceinline__ void copy_async(char* to, const char* from, bool on) {
-    const uint32_t d = static_cast<uint32_t>(__cvta_generic_to_shared(to));
+template <int BYTES> __device__ __forceinline__ void copy_async(uint32_t to, const char* from, bool on) {
     const int n = on ? BYTES : 0;
-    if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" :: "r"(d), "l"(from), "r"(n) : "memory");
-    else asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" :: "r"(d), "l"(from), "n"(BYTES), "r"(n) : "memory");
+    if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" :: "r"(to), "l"(from), "r"(n) : "memory");
+    else asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" :: "r"(to), "l"(from), "n"(BYTES), "r"(n) : "memory");
 }
+template <int WORDS> __device__ __forceinline__ void load_shared(uint32_t from, uint32_t (&w)[WORDS]) {
+    if constexpr (WORDS == 4) asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(from) : "memory");
+    else if constexpr (WORDS == 2) asm volatile("ld.shared.v2.b32 {%0,%1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(from) : "memory");
+    else asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w[0]) : "r"(from) : "memory");
+}
+// 2^x (2 ulp; results below 2^-126 become 0)
+__device__ __forceinline__ float exp2_fast(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
 __device__ __forceinline__ uint32_t half2_bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
 __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) { return half2_bits(__floats2half2_rn(lo, hi)); }
 
-template <int D, bool F8, bool WIDE, int STAGES>
+// 8 x 8 elements of 16 bits, a pair of a row a lane: transposed.
+__device__ __forceinline__ uint32_t transposed(uint32_t x) {
+    uint32_t y;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+// 2^(byte - top) for a scale byte that is at most top
+__device__ __forceinline__ float relative_scale(uint32_t byte, uint32_t top) { return __uint_as_float((uint32_t)max(127 + (int)byte - (int)top, 0) << 23); }
+
+template <int D, bool F8, int HT, int U, int STAGES>
 struct Cfg {
-    static constexpr int SZ = F8 ? 1 : 2;
+    static constexpr int SZ = F8 ? 1 : 2, ROW = 2 * D * SZ;              // bytes of an element, of a position
     static constexpr int KB = F8 ? (D % 64 == 0 ? 16 : 8) : 16;          // bytes of a piece of a key row: four lanes take 4 KB bytes
     static constexpr int KP = D * SZ / (4 * KB);                         // pieces a lane and key row
     static constexpr int VB = F8 ? (D % 128 == 0 ? 16 : D % 64 == 0 ? 8 : 4) : (D % 64 == 0 ? 16 : 8);     // of a value row: eight lanes take 8 VB
     static constexpr int VE = VB / SZ, VP = D / (8 * VE);                // elements of it, pieces a lane and value row
-    static constexpr int VOFF = 2 * KP * KB * 32;
-    static constexpr int SOFF = VOFF + 4 * VP * VB * 32;
-    static constexpr int STAGE = SOFF + (F8 ? 2 * 4 * 32 : 0);
-    static constexpr int ROWS = WIDE ? 16 : 8;
-    static constexpr int FIFO = kWarps * STAGES * STAGE, MERGE = kWarps * ROWS * (D + 2) * 4;
+    static constexpr int SOFF = kTile * ROW;                             // a tile's scale bytes behind its rows
+    static constexpr int STAGE = SOFF + (F8 ? 2 * kTile : 0);
+    static constexpr bool EXCHANGE = ROW % 128 == 0;                     // rows of whole 128-byte lines
+    static constexpr int HEADS = 8 * HT;
+    static constexpr int FIFO = kWarps * STAGES * U * STAGE, MERGE = kWarps * HEADS * (D + 2) * 4;
     static constexpr int BUF = FIFO > MERGE ? FIFO : MERGE;
     static constexpr int SMEM = BUF + 2 * D * SZ + 16;
-    static constexpr int NT = D / 8;                                     // n-tiles of the output
-    static constexpr int KS = D / 16;                                    // steps of the contraction over D
+    static constexpr int MT = D / 16;                                    // m-tiles of the output, and steps of the contraction over D
+
+    // Where a tile's byte `byte` of row `row` lies: pieces exchanged by s(row) in 0 .. 7.  The eight lanes of a read's phase ask for pieces x, .., x + 3 of two
+    // neighbouring rows (keys: bit 2 of s tells them apart) or two pieces of four rows two apart (values: bits 1 and 2).
+    __device__ static __forceinline__ int at(int row, int byte) {
+        return row * ROW + (EXCHANGE ? byte ^ ((row & 1) << 6 ^ (row >> 1 & 3) << 5) : byte);
+    }
 };
 
-template <int D, bool F8, bool WIDE, int STAGES, int CTAS>
+// U tiles a round, STAGES - 1 rounds of copies ahead.
+template <int D, bool F8, int HT, int U, int STAGES, int CTAS>
 __global__ void __launch_bounds__(kWarps * 32, CTAS) step_mma_kernel(const StepArgs a) {
-    using C = Cfg<D, F8, WIDE, STAGES>;
+    using C = Cfg<D, F8, HT, U, STAGES>;
     extern __shared__ __align__(16) char smem[];
     char* const fresh = smem + C::BUF;
     uint8_t* const fresh_scale = reinterpret_cast<uint8_t*>(fresh + 2 * D * C::SZ);
     stream_wait();
     const PageArgs& c = a.c;
-    const int blocks_h = (a.G + 15) / 16, hb = blockIdx.y % blocks_h, h = blockIdx.y / blocks_h, s = blockIdx.z, part = blockIdx.x;
+    const int blocks_h = (a.G + C::HEADS - 1) / C::HEADS, hb = blockIdx.y % blocks_h, h = blockIdx.y / blocks_h, s = blockIdx.z, part = blockIdx.x;
     const Range r = range_of(a, s, part);
     if (part && r.first >= r.length) return;                   // part 0 always answers
-    const int heads = min(16, a.G - hb * 16);
-    const long long q0 = ((long long)s * c.H + h) * a.G + hb * 16;
+    const int heads = min(C::HEADS, a.G - hb * C::HEADS);
+    const long long q0 = ((long long)s * c.H + h) * a.G + hb * C::HEADS;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const bool has_new = a.k_new != nullptr && r.end == r.length && r.length > 0;
     const int last = has_new ? r.length - 1 : -1, old_end = has_new ? r.length - 1 : r.end;     // rows in front of old_end come from the pages
 
-    char* const fifo = smem + warp * STAGES * C::STAGE;
-    const int first_tile = r.first + warp * kTile, tiles = r.end > first_tile ? (r.end - first_tile + kWarps * kTile - 1) / (kWarps * kTile) : 0;
+    const uint32_t fifo = static_cast<uint32_t>(__cvta_generic_to_shared(smem)) + warp * STAGES * U * C::STAGE;
+    constexpr int STEP = kWarps * kTile;                       // positions from a warp's tile to its next
+    const int first_tile = r.first + warp * kTile, tiles = r.end > first_tile ? (r.end - first_tile + STEP - 1) / STEP : 0;
     bool bad = r.bad;
 
-    const auto page_rows = [&](int i) -> long long {           // first row of tile i, -1: no page
-        const int p = first_tile + i * (kWarps * kTile);
-        if (i >= tiles) return 0;
-        const long long rows = c.rows_of(s, h, p / c.page);
-        return rows < 0 ? -1 : rows + p % c.page;
+    // ---- copies.  (column, row) of the table walk ahead of the tile that is asked for, so that the page's index is there when it is needed.
+    const int32_t* const table = c.table + (long long)s * c.columns;
+    const int step_columns = STEP / c.page, step_rows = STEP % c.page;
+    int walk = 0, column = first_tile / c.page, row = first_tile % c.page;
+    int next_id = 0, next_row = 0;
+    const auto look = [&] {                                    // the page of tile `walk`
+        if (walk < tiles) next_id = __ldg(table + column);
+        next_row = row;
+        ++walk; column += step_columns; row += step_rows;
+        if (row >= c.page) { row -= c.page; ++column; }
     };
-    const auto issue = [&](int i, long long row0) {
+    const auto issue = [&](int i, uint32_t st) {
+        const int id = next_id, row_in = next_row;
+        look();
         if (i < tiles) {
-            char* const st = fifo + (i % STAGES) * C::STAGE;
-            const int p = first_tile + i * (kWarps * kTile), n = row0 < 0 ? 0 : old_end - p;      // rows of the tile that exist
-            if (row0 < 0) { bad = true; row0 = 0; }
-            const char* const base = c.kv + row0 * (2 * D * C::SZ);
+            const bool there = id >= 0 && id < c.pages;
+            bad |= !there;
+            const int n = there ? old_end - (first_tile + i * STEP) : 0;         // rows of the tile that exist
+            const long long row0 = ((long long)(there ? id : 0) * c.H + h) * c.page + (there ? row_in : 0);
+            const char* const from = c.kv + row0 * C::ROW + lane * 16;
 #pragma unroll
-            for (int j = 0; j < 2; ++j)
-#pragma unroll
-                for (int k = 0; k < C::KP; ++k)
-                    copy_async<C::KB>(st + ((j * C::KP + k) * 32 + lane) * C::KB, base + (g + 8 * j) * (2 * D * C::SZ) + (4 * k + t) * C::KB, g + 8 * j < n);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int key = 2 * t + (j & 1) + 8 * (j >> 1);
-#pragma unroll
-                for (int k = 0; k < C::VP; ++k)
-                    copy_async<C::VB>(st + C::VOFF + ((j * C::VP + k) * 32 + lane) * C::VB, base + key * (2 * D * C::SZ) + D * C::SZ + (8 * k + g) * C::VB, key < n);
+            for (int j = 0; j < kTile * C::ROW / 512; ++j) {
+                const int byte = j * 512 + lane * 16, r = byte / C::ROW;
+                copy_async<16>(st + C::at(r, byte % C::ROW), from + j * 512, r < n);
             }
-            if constexpr (F8) {
-#pragma unroll
-                for (int j = 0; j < 2; ++j)
-                    copy_async<4>(st + C::SOFF + (j * 32 + lane) * 4, reinterpret_cast<const char*>(c.scale) + (row0 + 8 * j + 2 * t) * 2, true);
-            }
+            if constexpr (F8)
+                if (lane < kTile / 2) copy_async<4>(st + C::SOFF + lane * 4, reinterpret_cast<const char*>(c.scale) + row0 * 2 + lane * 4, true);
         }
+    };
+    const auto issue_round = [&](int first, int slot) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) issue(first + u, fifo + (slot * U + u) * C::STAGE);
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
-    long long next = page_rows(0);
+    look();
 #pragma unroll
-    for (int i = 0; i < STAGES - 1; ++i) {
-        const long long row0 = next;
-        next = page_rows(i + 1);
-        issue(i, row0);
-    }
+    for (int i = 0; i < STAGES - 1; ++i) issue_round(i * U, i);
 
-    // ---- queries as the A operand: registers 0 and 2 row g, 1 and 3 row g + 8
-    uint32_t qa[C::KS][4];
-    float fs[2] = {a.scale, a.scale};
+    // ---- queries as the B operand: column g of tile n
+    uint32_t qb[HT][C::MT][2];
+    float fs[HT][2];                                           // what the scores of columns 2 t, 2 t + 1 are multiplied by
     {
         const __nv_bfloat16* q = static_cast<const __nv_bfloat16*>(a.q) + q0 * D;
         constexpr int E = C::KB / C::SZ;                       // elements of a piece: E / 4 steps
 #pragma unroll
-        for (int row = 0; row < 2; ++row) {
-            const int hr = g + 8 * row;
-            const bool on = hr < heads && (WIDE || row == 0);
+        for (int n = 0; n < HT; ++n) {
+            const bool on = g + 8 * n < heads;
 #pragma unroll
             for (int k = 0; k < C::KP; ++k)
 #pragma unroll
                 for (int e = 0; e < E / 4; ++e) {
                     uint2 u = make_uint2(0u, 0u);
-                    if (on) u = *reinterpret_cast<const uint2*>(q + hr * D + (4 * k + t) * E + 4 * e);
-                    qa[k * (E / 4) + e][row] = u.x; qa[k * (E / 4) + e][2 + row] = u.y;
+                    if (on) u = *reinterpret_cast<const uint2*>(q + (g + 8 * n) * D + (4 * k + t) * E + 4 * e);
+                    qb[n][k * (E / 4) + e][0] = u.x; qb[n][k * (E / 4) + e][1] = u.y;
                 }
+            fs[n][0] = fs[n][1] = a.scale;
             if constexpr (F8) {
                 uint32_t top = 0u;
 #pragma unroll
-                for (int k = 0; k < C::KS; ++k)
+                for (int k = 0; k < C::MT; ++k)
 #pragma unroll
-                    for (int e = 0; e < 2; ++e) top = max(top, max(qa[k][row + 2 * e] << 16 & 0x7fff0000u, qa[k][row + 2 * e] & 0x7fff0000u));
+                    for (int e = 0; e < 2; ++e) top = max(top, max(qb[n][k][e] << 16 & 0x7fff0000u, qb[n][k][e] & 0x7fff0000u));
                 top = max(top, __shfl_xor_sync(0xffffffffu, top, 1)); top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
                 // largest element to [1, 2): nothing is lost but what is below 2^-25 of it.  NaN and infinity stay what they are.
                 int ex = (int)(top >> 23);
                 ex = ex == 0 ? 127 : ex >= 254 ? 253 : ex;
-                const float down = __uint_as_float((254u - ex) << 23);
-                fs[row] = a.scale * __uint_as_float((uint32_t)ex << 23);
+                const float down = __uint_as_float((254u - ex) << 23), up = a.scale * __uint_as_float((uint32_t)ex << 23);
 #pragma unroll
-                for (int k = 0; k < C::KS; ++k)
+                for (int k = 0; k < C::MT; ++k)
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
-                        uint32_t& w = qa[k][row + 2 * e];
+                        uint32_t& w = qb[n][k][e];
                         w = pack_f16x2(__uint_as_float(w << 16) * down, __uint_as_float(w & 0xffff0000u) * down);
                     }
+                fs[n][0] = __shfl_sync(0xffffffffu, up, 8 * t); fs[n][1] = __shfl_sync(0xffffffffu, up, 8 * t + 4);
             }
         }
     }
@@ -160,209 +190,222 @@ __global__ void __launch_bounds__(kWarps * 32, CTAS) step_mma_kernel(const StepA
         __syncthreads();
     }
 
-    float o[C::NT][4];
+    float o[HT][C::MT][4];
+    // m: what the exponentials are taken against, at least the running maximum less kSlack / fs; base: m fs, 0 where m is still -inf
+    float m[HT][2], l[HT][2], base[HT][2], lim[HT][2];
 #pragma unroll
-    for (int n = 0; n < C::NT; ++n)
+    for (int n = 0; n < HT; ++n) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) o[n][e] = 0.f;
-    constexpr int HALVES = WIDE ? 2 : 1;                       // rows g, and g + 8
-    float m[HALVES], l[HALVES];
+        for (int k = 0; k < C::MT; ++k)
 #pragma unroll
-    for (int i = 0; i < HALVES; ++i) { m[i] = -INFINITY; l[i] = 0.f; }
+            for (int e = 0; e < 4; ++e) o[n][k][e] = 0.f;
+        m[n][0] = m[n][1] = lim[n][0] = lim[n][1] = -INFINITY; l[n][0] = l[n][1] = base[n][0] = base[n][1] = 0.f;
+    }
     uint32_t vtop = 0u;                                        // largest scale byte of a value row so far
+    int slot = 0;
 
 #pragma unroll 1
-    for (int i = 0; i < tiles; ++i) {
-        {
-            const long long row0 = next;
-            next = page_rows(i + STAGES);
-            issue(i + STAGES - 1, row0);
-        }
+    for (int i = 0; i < tiles; i += U) {
+        __syncwarp();                                          // every lane has read the round that the next copies replace
+        issue_round(i + (STAGES - 1) * U, slot == 0 ? STAGES - 1 : slot - 1);
         asm volatile("cp.async.wait_group %0;" :: "n"(STAGES - 1) : "memory");
-        char* const st = fifo + (i % STAGES) * C::STAGE;
-        const int p = first_tile + i * (kWarps * kTile);
-        if (last >= p && last < p + kTile) {                   // the new token's row: from where new_row left it
-            const int key = last - p;
-            if (g == (key & 7)) {
-                const int j = key >> 3;
-#pragma unroll
-                for (int k = 0; k < C::KP; ++k)
-#pragma unroll
-                    for (int b = 0; b < C::KB; b += 8)
-                        *reinterpret_cast<uint2*>(st + ((j * C::KP + k) * 32 + lane) * C::KB + b) = *reinterpret_cast<const uint2*>(fresh + (4 * k + t) * C::KB + b);
-            }
-            if (t == (key & 7) >> 1) {
-                const int j = (key & 1) + 2 * (key >> 3);
-#pragma unroll
-                for (int k = 0; k < C::VP; ++k)
-#pragma unroll
-                    for (int b = 0; b < C::VB; b += 4)
-                        *reinterpret_cast<uint32_t*>(st + C::VOFF + ((j * C::VP + k) * 32 + lane) * C::VB + b) =
-                            *reinterpret_cast<const uint32_t*>(fresh + D * C::SZ + (8 * k + g) * C::VB + b);
-                if constexpr (F8) {
-                    uint8_t* b = reinterpret_cast<uint8_t*>(st + C::SOFF + ((key >> 3) * 32 + lane) * 4) + 2 * (key & 1);
-                    b[0] = fresh_scale[0]; b[1] = fresh_scale[1];
-                }
-            }
+        __syncwarp();
+        const uint32_t st0 = fifo + slot * U * C::STAGE;
+        slot = slot == STAGES - 1 ? 0 : slot + 1;
+        const int p0 = first_tile + i * STEP;                  // tile u of the round: positions p0 + u STEP on
+        if (last >= p0 && last < p0 + (U - 1) * STEP + kTile && (last - p0) % STEP < kTile) {      // the new token's row: from where new_row left it
+            const int key = (last - p0) % STEP;
+            char* const to = smem + (st0 - static_cast<uint32_t>(__cvta_generic_to_shared(smem))) + (last - p0) / STEP * C::STAGE;
+            if (lane * 16 < C::ROW) *reinterpret_cast<uint4*>(to + C::at(key, lane * 16)) = *reinterpret_cast<const uint4*>(fresh + lane * 16);
+            if (F8 && lane < 2) to[C::SOFF + 2 * key + lane] = fresh_scale[lane];
+            __syncwarp();
         }
-        // ---- scores of 16 positions: column 2 t and 2 t + 1 of each half
-        float sc[2][4];
+        // ---- scores: positions g and g + 8 of a tile, heads 2 t and 2 t + 1; two chains of products each, for they wait for one another
+        float sc[U][HT][4];
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
+        for (int u = 0; u < U; ++u) {
+            const uint32_t st = st0 + u * C::STAGE;
+            float odd[HT][4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) sc[j][e] = 0.f;
+            for (int n = 0; n < HT; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) sc[u][n][e] = odd[n][e] = 0.f;
 #pragma unroll
             for (int k = 0; k < C::KP; ++k) {
-                uint32_t w[C::KB / 4];
-                const char* from = st + ((j * C::KP + k) * 32 + lane) * C::KB;
-                if constexpr (C::KB == 16) { const uint4 u = *reinterpret_cast<const uint4*>(from); w[0] = u.x; w[1] = u.y; w[2] = u.z; w[3] = u.w; }
-                else { const uint2 u = *reinterpret_cast<const uint2*>(from); w[0] = u.x; w[1] = u.y; }
-                if constexpr (F8) {
+                uint32_t w[2][C::KB / 4];
+                load_shared(st + C::at(g, (4 * k + t) * C::KB), w[0]);
+                load_shared(st + C::at(g, (4 * k + t) * C::KB) + 8 * C::ROW, w[1]);      // s(g + 8) = s(g)
+                constexpr int N = F8 ? C::KB / 4 : 2;          // steps of a piece
 #pragma unroll
-                    for (int e = 0; e < C::KB / 4; ++e)
-                        mma<true>(sc[j], qa[k * (C::KB / 4) + e], half2_bits(e4m3x2_half2(w[e] & 0xffffu)), half2_bits(e4m3x2_half2(w[e] >> 16)));
-                } else {
-                    mma<false>(sc[j], qa[2 * k], w[0], w[1]);
-                    mma<false>(sc[j], qa[2 * k + 1], w[2], w[3]);
+                for (int e = 0; e < N; ++e) {
+                    uint32_t ka[4];
+                    if constexpr (F8) { e4m3x4_half2(w[0][e], ka[0], ka[2]); e4m3x4_half2(w[1][e], ka[1], ka[3]); }
+                    else { ka[0] = w[0][2 * e]; ka[1] = w[1][2 * e]; ka[2] = w[0][2 * e + 1]; ka[3] = w[1][2 * e + 1]; }
+#pragma unroll
+                    for (int n = 0; n < HT; ++n) mma<F8>(e & 1 ? odd[n] : sc[u][n], ka, qb[n][k * N + e][0], qb[n][k * N + e][1]);
                 }
             }
-        }
-        // ---- softmax: the scale bytes of positions 2 t, 2 t + 1 (+ 8) are {k, v, k, v}
-        uint32_t sb[2];
-        bool valid[2][2];
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            if constexpr (F8) sb[j] = *reinterpret_cast<const uint32_t*>(st + C::SOFF + (j * 32 + lane) * 4);
+            for (int n = 0; n < HT; ++n)
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                valid[j][e] = p + 8 * j + 2 * t + e < r.end;
-                if constexpr (F8) {
-                    const float ks = scale_value(sb[j] >> (16 * e) & 255u);
-                    sc[j][e] *= ks; sc[j][2 + e] *= ks;
-                }
-            }
+                for (int e = 0; e < 4; ++e) sc[u][n][e] += odd[n][e];
         }
-        float vs[2][2];
+        // ---- softmax.  A score is the product times its row's scale (ks), in units of 1 / fs; m is in the same units.
+        bool valid[U][2];
+        float ks[U][2], vs[U][2];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) { valid[u][j] = p0 + u * STEP + 8 * j + g < r.end; ks[u][j] = vs[u][j] = 1.f; }
         if constexpr (F8) {
-            uint32_t top = 0u;
+            uint32_t kb[U][2], vb[U][2], top = 0u;
+            bool nan = false;
 #pragma unroll
-            for (int j = 0; j < 2; ++j)
+            for (int u = 0; u < U; ++u)
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const uint32_t b = sb[j] >> (16 * e + 8) & 255u;
-                    if (valid[j][e] && b != 255u) top = max(top, b);
+                for (int j = 0; j < 2; ++j) {
+                    uint16_t b;
+                    asm volatile("ld.shared.u16 %0, [%1];" : "=h"(b) : "r"(st0 + u * C::STAGE + C::SOFF + 2 * (8 * j + g)) : "memory");
+                    if (!valid[u][j]) b = 0;
+                    kb[u][j] = b & 255u; vb[u][j] = b >> 8;
+                    nan |= kb[u][j] == 255u || vb[u][j] == 255u;
+                    top = max(top, vb[u][j]);
+                    ks[u][j] = __uint_as_float(kb[u][j] << 23);               // a byte of 0 (2^-127, which no row of this library has): 0
                 }
+            const bool some_nan = __any_sync(0xffffffffu, nan);
+            if (some_nan) {
+                top = 0u;
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) top = max(top, vb[u][j] == 255u ? 0u : vb[u][j]);
+            }
             top = __reduce_max_sync(0xffffffffu, top);
             if (top > vtop) {                                  // rarely: the scales of a head's values are much alike
-                const int e = 127 + (int)vtop - (int)top;
-                const float f = e > 0 ? __uint_as_float((uint32_t)e << 23) : 0.f;
+                const float f = relative_scale(vtop, top);
 #pragma unroll
-                for (int n = 0; n < C::NT; ++n)
+                for (int n = 0; n < HT; ++n)
 #pragma unroll
-                    for (int x = 0; x < 4; ++x) o[n][x] *= f;
+                    for (int k = 0; k < C::MT; ++k)
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) o[n][k][x] *= f;
                 vtop = top;
             }
 #pragma unroll
-            for (int j = 0; j < 2; ++j)
+            for (int u = 0; u < U; ++u)
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const uint32_t b = sb[j] >> (16 * e + 8) & 255u;
-                    const int x = 127 + (int)b - (int)vtop;
-                    vs[j][e] = !valid[j][e] ? 0.f : b == 255u ? __uint_as_float(0x7fc00000u) : x > 0 ? __uint_as_float((uint32_t)x << 23) : 0.f;
+                for (int j = 0; j < 2; ++j) {
+                    vs[u][j] = relative_scale(vb[u][j], vtop);
+                    if (some_nan) {
+                        if (kb[u][j] == 255u) ks[u][j] = __uint_as_float(0x7fc00000u);
+                        if (vb[u][j] == 255u) vs[u][j] = __uint_as_float(0x7fc00000u);
+                    }
                 }
         }
-        uint32_t pa[4] = {0u, 0u, 0u, 0u};
+        uint32_t pb[U][HT][2];
 #pragma unroll
-        for (int i2 = 0; i2 < HALVES; ++i2) {
-            float mx = -INFINITY;
+        for (int n = 0; n < HT; ++n) {
+            float mx[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-            for (int j = 0; j < 2; ++j)
+            for (int u = 0; u < U; ++u)
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    float& x = sc[j][2 * i2 + e];
-                    x = valid[j][e] ? x * fs[i2] : -INFINITY;
-                    mx = fmaxf(mx, x);
+                for (int x = 0; x < 2; ++x)
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        float& v = sc[u][n][2 * j + x];
+                        if constexpr (F8) v *= ks[u][j];
+                        v = valid[u][j] ? v : -INFINITY;
+                        mx[x] = fmaxf(mx[x], v);
+                    }
+            if (__any_sync(0xffffffffu, mx[0] > lim[n][0] || mx[1] > lim[n][1])) {
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+#pragma unroll
+                    for (int b = 4; b < 32; b <<= 1) mx[x] = fmaxf(mx[x], __shfl_xor_sync(0xffffffffu, mx[x], b));
+                    const float mn = fmaxf(m[n][x], mx[x]), f = mn == -INFINITY ? 1.f : exp2_fast((m[n][x] - mn) * fs[n][x]);
+                    m[n][x] = mn;
+                    lim[n][x] = mn + kSlack / fs[n][x];
+                    base[n][x] = mn == -INFINITY ? 0.f : mn * fs[n][x];
+                    l[n][x] *= f;
+#pragma unroll
+                    for (int k = 0; k < C::MT; ++k) { o[n][k][x] *= f; o[n][k][2 + x] *= f; }
                 }
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1)); mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-            if (__any_sync(0xffffffffu, mx > m[i2])) {
-                const float mn = fmaxf(m[i2], mx), f = mn == -INFINITY ? 1.f : exp2f(m[i2] - mn);
-                l[i2] *= f;
-#pragma unroll
-                for (int n = 0; n < C::NT; ++n) { o[n][2 * i2] *= f; o[n][2 * i2 + 1] *= f; }
-                m[i2] = mn;
             }
-            const float base = m[i2] == -INFINITY ? 0.f : m[i2];
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                float x[2];
+            for (int u = 0; u < U; ++u)
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    x[e] = exp2f(sc[j][2 * i2 + e] - base);
-                    l[i2] += x[e];
-                    if constexpr (F8) x[e] *= vs[j][e];
+                for (int j = 0; j < 2; ++j) {
+                    float x[2];
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        x[e] = exp2_fast(fmaf(sc[u][n][2 * j + e], fs[n][e], -base[n][e]));
+                        l[n][e] += x[e];
+                        if constexpr (F8) x[e] *= vs[u][j];
+                    }
+                    // to 16 bits, as the operand of the product: relative 2^-9 (bf16) or 2^-12 (f16) on terms that add up, within the result's own rounding
+                    pb[u][n][j] = transposed(F8 ? pack_f16x2(x[0], x[1]) : pack_bf16x2(x[0], x[1]));
                 }
-                // to 16 bits, as the operand of the product: relative 2^-9 (bf16) or 2^-12 (f16) on terms that add up, within the result's own rounding
-                pa[2 * j + i2] = F8 ? pack_f16x2(x[0], x[1]) : pack_bf16x2(x[0], x[1]);
-            }
         }
-        // ---- O += P V: n-tile k VE + e has column n at d = 8 VE k + VE n + e
+        // ---- O^T += V^T P^T: rows g and g + 8 of m-tile (k VE + e) / 2 are d = 8 VE k + VE g + e and the next
 #pragma unroll
-        for (int k = 0; k < C::VP; ++k) {
-            uint32_t w[4][C::VB / 4];
+        for (int u = 0; u < U; ++u)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const char* from = st + C::VOFF + ((j * C::VP + k) * 32 + lane) * C::VB;
-                if constexpr (C::VB == 16) { const uint4 u = *reinterpret_cast<const uint4*>(from); w[j][0] = u.x; w[j][1] = u.y; w[j][2] = u.z; w[j][3] = u.w; }
-                else if constexpr (C::VB == 8) { const uint2 u = *reinterpret_cast<const uint2*>(from); w[j][0] = u.x; w[j][1] = u.y; }
-                else w[j][0] = *reinterpret_cast<const uint32_t*>(from);
+            for (int k = 0; k < C::VP; ++k) {
+                uint32_t w[4][C::VB / 4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j)                    // positions 2 t, 2 t + 1 (+ 8)
+                    load_shared(st0 + u * C::STAGE + C::at(2 * t + (j & 1), D * C::SZ + (8 * k + g) * C::VB) + 8 * (j >> 1) * C::ROW, w[j]);
+#pragma unroll
+                for (int x = 0; x < C::VB / 4; ++x) {
+                    if constexpr (F8) {
+#pragma unroll
+                        for (int y = 0; y < 2; ++y) {          // columns 2 y, 2 y + 1 of the word: {position, next position} of each
+                            uint32_t va[4];
+                            e4m3x4_half2(__byte_perm(w[0][x], w[1][x], y ? 0x7362 : 0x5140), va[0], va[1]);
+                            e4m3x4_half2(__byte_perm(w[2][x], w[3][x], y ? 0x7362 : 0x5140), va[2], va[3]);
+#pragma unroll
+                            for (int n = 0; n < HT; ++n) mma<true>(o[n][(k * C::VE + 4 * x) / 2 + y], va, pb[u][n][0], pb[u][n][1]);
+                        }
+                    } else {
+                        const uint32_t va[4] = {__byte_perm(w[0][x], w[1][x], 0x5410), __byte_perm(w[0][x], w[1][x], 0x7632),
+                                                __byte_perm(w[2][x], w[3][x], 0x5410), __byte_perm(w[2][x], w[3][x], 0x7632)};
+#pragma unroll
+                        for (int n = 0; n < HT; ++n) mma<false>(o[n][(k * C::VE + 2 * x) / 2], va, pb[u][n][0], pb[u][n][1]);
+                    }
+                }
             }
-            // pairs of columns of four positions -> the B operands of two n-tiles
-            const auto two = [&](int n, uint32_t w0, uint32_t w1, uint32_t w2, uint32_t w3) {
-                mma<F8>(o[n], pa, __byte_perm(w0, w1, 0x5410), __byte_perm(w2, w3, 0x5410));
-                mma<F8>(o[n + 1], pa, __byte_perm(w0, w1, 0x7632), __byte_perm(w2, w3, 0x7632));
-            };
-#pragma unroll
-            for (int x = 0; x < C::VB / 4; ++x) {
-                if constexpr (F8) {
-                    two(k * C::VE + 4 * x, half2_bits(e4m3x2_half2(w[0][x] & 0xffffu)), half2_bits(e4m3x2_half2(w[1][x] & 0xffffu)),
-                        half2_bits(e4m3x2_half2(w[2][x] & 0xffffu)), half2_bits(e4m3x2_half2(w[3][x] & 0xffffu)));
-                    two(k * C::VE + 4 * x + 2, half2_bits(e4m3x2_half2(w[0][x] >> 16)), half2_bits(e4m3x2_half2(w[1][x] >> 16)),
-                        half2_bits(e4m3x2_half2(w[2][x] >> 16)), half2_bits(e4m3x2_half2(w[3][x] >> 16)));
-                } else two(k * C::VE + 2 * x, w[0][x], w[1][x], w[2][x], w[3][x]);
-            }
-        }
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
     // ---- the four warps' results, joined in warp order
     const bool any_bad = __syncthreads_or(bad);
-    float* const sml = reinterpret_cast<float*>(smem);         // [warps][rows][2]
-    float* const so = sml + kWarps * C::ROWS * 2;              // [warps][rows][D]
+    float* const sml = reinterpret_cast<float*>(smem);         // [warps][heads][2]
+    float* const so = sml + kWarps * C::HEADS * 2;             // [warps][heads][D]
     const float unit = F8 ? scale_value(vtop) : 1.f;
 #pragma unroll
-    for (int i = 0; i < HALVES; ++i) {
-        const int row = g + 8 * i;
-        l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1); l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
-        if (t == 0) { sml[(warp * C::ROWS + row) * 2] = m[i]; sml[(warp * C::ROWS + row) * 2 + 1] = l[i]; }
+    for (int n = 0; n < HT; ++n)
 #pragma unroll
-        for (int k = 0; k < C::VP; ++k)
+        for (int x = 0; x < 2; ++x) {
+            const int at = warp * C::HEADS + 8 * n + 2 * t + x;
 #pragma unroll
-            for (int e = 0; e < C::VE; ++e)
+            for (int b = 4; b < 32; b <<= 1) l[n][x] += __shfl_xor_sync(0xffffffffu, l[n][x], b);
+            if (g == 0) { sml[at * 2] = m[n][x] == -INFINITY ? -INFINITY : base[n][x]; sml[at * 2 + 1] = l[n][x]; }
 #pragma unroll
-                for (int x = 0; x < 2; ++x)
-                    so[(warp * C::ROWS + row) * D + 8 * C::VE * k + C::VE * (2 * t + x) + e] = o[k * C::VE + e][2 * i + x] * unit;
-    }
+            for (int k = 0; k < C::VP; ++k)
+#pragma unroll
+                for (int e = 0; e < C::VE; ++e) so[at * D + 8 * C::VE * k + C::VE * g + e] = o[n][(k * C::VE + e) / 2][2 * (e & 1) + x] * unit;
+        }
     __syncthreads();
     for (int z = threadIdx.x; z < heads * D; z += kWarps * 32) {
         const int row = z / D, d = z - row * D;
         float M = -INFINITY;
 #pragma unroll
-        for (int w = 0; w < kWarps; ++w) M = fmaxf(M, sml[(w * C::ROWS + row) * 2]);
+        for (int w = 0; w < kWarps; ++w) M = fmaxf(M, sml[(w * C::HEADS + row) * 2]);
         const float base = M == -INFINITY ? 0.f : M;
         float L = 0.f, A = 0.f;
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) {
-            const float f = exp2f(sml[(w * C::ROWS + row) * 2] - base);
-            L = fmaf(f, sml[(w * C::ROWS + row) * 2 + 1], L); A = fmaf(f, so[(w * C::ROWS + row) * D + d], A);
+            const float f = exp2f(sml[(w * C::HEADS + row) * 2] - base);
+            L = fmaf(f, sml[(w * C::HEADS + row) * 2 + 1], L); A = fmaf(f, so[(w * C::HEADS + row) * D + d], A);
         }
         if (any_bad) L = A = __uint_as_float(0x7fc00000u);
         if (a.ml) {
@@ -373,9 +416,9 @@ __global__ void __launch_bounds__(kWarps * 32, CTAS) step_mma_kernel(const StepA
     }
 }
 
-template <int D, bool F8, bool WIDE, int STAGES, int CTAS> cudaError_t launch_one(const StepArgs& a, cudaStream_t s) {
-    using C = Cfg<D, F8, WIDE, STAGES>;
-    auto kern = step_mma_kernel<D, F8, WIDE, STAGES, CTAS>;
+template <int D, bool F8, int HT, int U, int STAGES, int CTAS> cudaError_t launch_one(const StepArgs& a, cudaStream_t s) {
+    using C = Cfg<D, F8, HT, U, STAGES>;
+    auto kern = step_mma_kernel<D, F8, HT, U, STAGES, CTAS>;
     static bool ready[64] = {};                                // per device: the attribute is set once
     int dev = 0;
     if (cudaError_t e = cudaGetDevice(&dev)) return e;
@@ -383,11 +426,13 @@ template <int D, bool F8, bool WIDE, int STAGES, int CTAS> cudaError_t launch_on
         if (cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM)) { cudaGetLastError(); return e; }
         if (dev >= 0 && dev < 64) ready[dev] = true;
     }
-    return launch_after(kern, dim3(a.parts, a.c.H * ((a.G + 15) / 16), a.c.S), kWarps * 32, C::SMEM, s, a);
+    return launch_after(kern, dim3(a.parts, a.c.H * ((a.G + C::HEADS - 1) / C::HEADS), a.c.S), kWarps * 32, C::SMEM, s, a);
 }
 template <int D, bool F8> cudaError_t launch_width(const StepArgs& a, cudaStream_t s) {
-    constexpr int STAGES = F8 ? 4 : D > 64 ? 3 : 4;
-    return a.G > 8 ? launch_one<D, F8, true, STAGES, 2>(a, s) : launch_one<D, F8, false, STAGES, 2>(a, s);
+    // Two CTAs of four warps and 8-KB tiles in bf16, four in 8 bits, two tiles ahead each (us, 64 sequences up to 4096, 8 x 4 heads of 128 in bf16 / 4 up to
+    // 100001, 4 x 8 heads of 128 in 8 bits: 90.9 / 59.6; one tile ahead and three CTAs 91.5 / 67.8; two tiles a round, three CTAs, 8 bits 67.8).
+    if (a.G > 8) return launch_one<D, F8, 2, 1, 3, 2>(a, s);
+    return launch_one<D, F8, 1, 1, 3, F8 ? 4 : 2>(a, s);
 }
 template <bool F8> cudaError_t launch_type(const StepArgs& a, cudaStream_t s) {
     switch (a.c.D) {

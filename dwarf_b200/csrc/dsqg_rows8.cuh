@@ -40,6 +40,10 @@ __device__ __forceinline__ __half2 e4m3x2_half2(uint32_t two) {
     const __half2_raw r = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)two, __NV_E4M3);
     return __half2(r);
 }
+// four of them as two half2, in the bits of 32-bit words
+__device__ __forceinline__ void e4m3x4_half2(uint32_t w, uint32_t& lo, uint32_t& hi) {
+    asm("{.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;}" : "=r"(lo), "=r"(hi) : "r"(w));
+}
 __device__ __forceinline__ void e4m3x4_float(uint32_t w, float* x) {
     const float2 a = __half22float2(e4m3x2_half2(w & 0xffffu)), b = __half22float2(e4m3x2_half2(w >> 16));
     x[0] = a.x; x[1] = a.y; x[2] = b.x; x[3] = b.y;
