@@ -1,9 +1,12 @@
 // Single-token DSQG decode over rings in 8 bits: e4m3 rows with a power-of-two scale each (dsqg_rows8.cuh), key and value of a slot side by side.
 //
-// As csrc/dsqg_decode.cu: one warp per (sequence, head), a group of TPR lanes takes a tap, every row of up to R rounds of taps is requested before
-// one is used.  A row is half as long as in bf16, so a lane holds twice the elements in the same load and a round covers twice the taps: 43 taps of
-// 64 columns are six rounds of 16-byte loads, which registers hold (bf16 needs eleven, most of them in shared memory).  The step attends to what the ring
-// holds: the new token's rows are quantised first, and tap 0 reads them.
+// As csrc/dsqg_decode.cu: one warp per (sequence, head), a group of TPR lanes takes a tap, every row of up to R rounds of taps is requested before one is
+// used: with cp.async into shared memory, no register held while in flight, and each lane reads back only the bytes it requested itself, so no barrier is
+// needed after the wait.  A row is half as long as in bf16, so a lane holds twice the elements in the same load and a round covers twice the taps: 43 taps
+// of 64 columns are six rounds.  The step attends to what the ring holds: the new token's rows are quantised first, and tap 0 reads them.
+//
+// 256 sequences, 12 heads of 64, 43 taps: HBM's floor is 2.9 us, the dependent chain of one wave of warps (write head, rows, softmax, result) the rest.
+// With the rows of a step in registers (157 of them, 12 warps an SM, two waves) it took 10.6.
 #include "dsqg_rows8.cuh"
 
 namespace dsqg {
@@ -11,25 +14,34 @@ namespace {
 
 constexpr int kWarps = 4;
 
-template <int VEC> struct Bytes;                               // VEC e4m3 values of a row
-template <> struct Bytes<16> {
-    uint4 u;
-    __device__ __forceinline__ void load(const uint8_t* p) { u = *reinterpret_cast<const uint4*>(p); }
-    __device__ __forceinline__ void store(uint8_t* p) const { *reinterpret_cast<uint4*>(p) = u; }
-    __device__ __forceinline__ void zero() { u = make_uint4(0u, 0u, 0u, 0u); }
-    __device__ __forceinline__ void get(float (&x)[16]) const { e4m3x4_float(u.x, x); e4m3x4_float(u.y, x + 4); e4m3x4_float(u.z, x + 8); e4m3x4_float(u.w, x + 12); }
-    __device__ __forceinline__ void set(const float (&x)[16]) {
-        u = make_uint4(pack_e4m3x4(x[0], x[1], x[2], x[3]), pack_e4m3x4(x[4], x[5], x[6], x[7]), pack_e4m3x4(x[8], x[9], x[10], x[11]), pack_e4m3x4(x[12], x[13], x[14], x[15]));
+template <int VEC> struct Bytes {                               // VEC e4m3 values of a row (to load and store: 8 or 16)
+    uint32_t u[VEC / 4];
+    __device__ __forceinline__ void load(const void* p) {
+        if constexpr (VEC == 16) { const uint4 v = *static_cast<const uint4*>(p); u[0] = v.x; u[1] = v.y; u[2] = v.z; u[3] = v.w; }
+        else { const uint2 v = *static_cast<const uint2*>(p); u[0] = v.x; u[1] = v.y; }
+    }
+    __device__ __forceinline__ void store(void* p) const {
+        if constexpr (VEC == 16) *static_cast<uint4*>(p) = make_uint4(u[0], u[1], u[2], u[3]);
+        else *static_cast<uint2*>(p) = make_uint2(u[0], u[1]);
+    }
+    __device__ __forceinline__ f32x2 get(int i) const {        // values 2 i, 2 i + 1
+        const float2 v = __half22float2(e4m3x2_half2(i & 1 ? u[i / 2] >> 16 : u[i / 2] & 0xffffu));
+        return pair(v.x, v.y);
+    }
+    __device__ __forceinline__ void set(const float (&x)[VEC]) {
+#pragma unroll
+        for (int i = 0; i < VEC / 4; ++i) u[i] = pack_e4m3x4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
     }
 };
-template <> struct Bytes<8> {
-    uint2 u;
-    __device__ __forceinline__ void load(const uint8_t* p) { u = *reinterpret_cast<const uint2*>(p); }
-    __device__ __forceinline__ void store(uint8_t* p) const { *reinterpret_cast<uint2*>(p) = u; }
-    __device__ __forceinline__ void zero() { u = make_uint2(0u, 0u); }
-    __device__ __forceinline__ void get(float (&x)[8]) const { e4m3x4_float(u.x, x); e4m3x4_float(u.y, x + 4); }
-    __device__ __forceinline__ void set(const float (&x)[8]) { u = make_uint2(pack_e4m3x4(x[0], x[1], x[2], x[3]), pack_e4m3x4(x[4], x[5], x[6], x[7])); }
-};
+// BYTES from global to shared memory, zeros where `on` is false
+template <int BYTES> __device__ __forceinline__ void copy_async(void* to, const void* from, bool on) {
+    const uint32_t d = static_cast<uint32_t>(__cvta_generic_to_shared(to));
+    const int n = on ? BYTES : 0;
+    if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" :: "r"(d), "l"(from), "r"(n) : "memory");
+    else asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" :: "r"(d), "l"(from), "n"(BYTES), "r"(n) : "memory");
+}
+// scale_value of a byte from 1 on (0, which no row of this library has: 0)
+__device__ __forceinline__ float row_scale(uint32_t byte) { return byte == 255u ? __uint_as_float(0x7fc00000u) : __uint_as_float(byte << 23); }
 template <typename T, int VEC> __device__ __forceinline__ void load_row(const void* p, long long i, float (&x)[VEC]) {
 #pragma unroll
     for (int b = 0; b < VEC; b += 8) {
@@ -54,10 +66,11 @@ template <int TPR, int VEC> __device__ __forceinline__ uint32_t quantize(float (
 
 // T: type of q, k_new, v_new, out.  PDL: the overlapped form (dsqg_decode.cu), which reads head, fill and the rows of taps with delta > 0 before it waits.
 template <typename T, int TPR, int VEC, int R, bool PDL>
-__global__ void __launch_bounds__(kWarps * 32)
+__global__ void __launch_bounds__(kWarps * 32, 6)
 decode8_kernel(const DecodeArgs a, uint8_t* __restrict__ scale, const Taps t) {
     if constexpr (!PDL) stream_wait();
     constexpr int GROUPS = 32 / TPR;
+    __shared__ __align__(16) char rows[kWarps][R][2][32 * VEC];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int sh = blockIdx.x * kWarps + warp;                 // (sequence, head) pair
     if (sh >= a.S * a.H) return;                               // whole warp leaves together
@@ -68,15 +81,13 @@ decode8_kernel(const DecodeArgs a, uint8_t* __restrict__ scale, const Taps t) {
     uint8_t* const ring = static_cast<uint8_t*>(a.k_ring) + (size_t)sh * a.R * 2 * D;
     uint8_t* const bytes = scale + (size_t)sh * a.R * 2;
 
-    float q[VEC], acc[VEC], m = -INFINITY, l = 0.f;
+    f32x2 q[VEC / 2], acc[VEC / 2];
+    float m = -INFINITY, l = 0.f;
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) acc[e] = q[e] = 0.f;
-    Bytes<VEC> kn, vn;
-    uint32_t new_scale = 0u;
+    for (int e = 0; e < VEC / 2; ++e) acc[e] = q[e] = pair(0.f, 0.f);
     const int rounds = (t.J + GROUPS - 1) / GROUPS;
 #pragma unroll 1
     for (int r0 = 0; r0 < rounds; r0 += R) {                   // one pass for the usual tap counts
-        Bytes<VEC> k[R], v[R];
         uint32_t sb[R];
         unsigned exists = 0u;
 #pragma unroll
@@ -85,52 +96,62 @@ decode8_kernel(const DecodeArgs a, uint8_t* __restrict__ scale, const Taps t) {
             const int delta = j < t.J ? t.delta(j) : 0;
             int slot = head - delta;
             if (slot < 0) slot += a.R;
-            k[r].zero(); v[r].zero(); sb[r] = 127u | 127u << 8;
-            if (j < t.J && delta < fill) {
-                exists |= 1u << r;
-                if (delta) {
-                    if (active) { k[r].load(ring + (size_t)slot * 2 * D + d0); v[r].load(ring + (size_t)slot * 2 * D + D + d0); }
-                    sb[r] = *reinterpret_cast<const uint16_t*>(bytes + 2 * slot);
-                }
-            }
+            const bool tap = j < t.J && delta < fill;
+            if (tap) exists |= 1u << r;
+            const bool old = tap && delta > 0;
+            const uint8_t* const from = ring + (size_t)(old && active ? slot : 0) * 2 * D + (active ? d0 : 0);
+            copy_async<VEC>(&rows[warp][r][0][lane * VEC], from, old && active);
+            copy_async<VEC>(&rows[warp][r][1][lane * VEC], from + D, old && active);
+            sb[r] = 127u | 127u << 8;
+            if (old) sb[r] = *reinterpret_cast<const uint16_t*>(bytes + 2 * slot);
         }
         if (r0 == 0) {
             if constexpr (PDL) stream_wait();
-            float x[VEC];
+            float x[VEC], y[VEC], z[VEC];
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) x[e] = 0.f;
-            if (active) load_row<T, VEC>(a.k_new, (long long)sh * D + d0, x);
-            float y[VEC];
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) y[e] = 0.f;
-            if (active) { load_row<T, VEC>(a.v_new, (long long)sh * D + d0, y); load_row<T, VEC>(a.q, (long long)sh * D + d0, q); }
-            new_scale = quantize<TPR, VEC>(x, kn);
-            new_scale |= quantize<TPR, VEC>(y, vn) << 8;
-            if (g == 0 && active) {                            // the new token's slot
-                kn.store(ring + (size_t)head * 2 * D + d0); vn.store(ring + (size_t)head * 2 * D + D + d0);
-                if (d0 == 0) *reinterpret_cast<uint16_t*>(bytes + 2 * head) = (uint16_t)new_scale;
+            for (int e = 0; e < VEC; ++e) x[e] = y[e] = z[e] = 0.f;
+            if (active) {
+                load_row<T, VEC>(a.k_new, (long long)sh * D + d0, x); load_row<T, VEC>(a.v_new, (long long)sh * D + d0, y);
+                load_row<T, VEC>(a.q, (long long)sh * D + d0, z);
             }
-            if (g == 0 && t.delta(0) == 0 && (exists & 1u)) { k[0] = kn; v[0] = vn; sb[0] = new_scale; }      // offsets ascend: only tap 0 can be delta 0
-        }
+#pragma unroll
+            for (int e = 0; e < VEC / 2; ++e) q[e] = pair(z[2 * e], z[2 * e + 1]);
+            Bytes<VEC> kn, vn;
+            uint32_t new_scale = quantize<TPR, VEC>(x, kn);
+            new_scale |= quantize<TPR, VEC>(y, vn) << 8;
+            asm volatile("cp.async.wait_all;" ::: "memory");
+            if (g == 0) {
+                if (active) {                                  // the new token's slot
+                    kn.store(ring + (size_t)head * 2 * D + d0); vn.store(ring + (size_t)head * 2 * D + D + d0);
+                    if (d0 == 0) *reinterpret_cast<uint16_t*>(bytes + 2 * head) = (uint16_t)new_scale;
+                }
+                if (t.delta(0) == 0 && (exists & 1u)) {        // offsets ascend: only tap 0 can be delta 0
+                    kn.store(&rows[warp][0][0][lane * VEC]); vn.store(&rows[warp][0][1][lane * VEC]);
+                    sb[0] = new_scale;
+                }
+            }
+        } else asm volatile("cp.async.wait_all;" ::: "memory");
         // ---- scores of the pass, then one softmax step over all of them
         float sc[R];
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-            float x[VEC];
-            k[r].get(x);
-            const int j = (r0 + r) * GROUPS + g;
-            const float ks = scale_value(sb[r] & 255u);
-            float dot = 0.f;
+            Bytes<VEC> k;
+            k.load(&rows[warp][r][0][lane * VEC]);
+            f32x2 dot = pair(0.f, 0.f);
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) dot = fmaf(q[e], x[e], dot);
-            dot *= ks;
+            for (int e = 0; e < VEC / 2; ++e) dot = fma2(q[e], k.get(e), dot);
+            float lo, hi;
+            unpair(dot, lo, hi);
+            sc[r] = (lo + hi) * row_scale(sb[r] & 255u);
             if (a.scale_embed != nullptr && (exists >> r & 1u) && active) {
                 float se[VEC];
-                load_row<float, VEC>(a.scale_embed, (long long)j * D + d0, se);
+                load_row<float, VEC>(a.scale_embed, (long long)((r0 + r) * GROUPS + g) * D + d0, se);
+                dot = pair(0.f, 0.f);
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) dot = fmaf(q[e], se[e], dot);
+                for (int e = 0; e < VEC / 2; ++e) dot = fma2(q[e], pair(se[2 * e], se[2 * e + 1]), dot);
+                unpair(dot, lo, hi);
+                sc[r] += lo + hi;
             }
-            sc[r] = dot;
         }
 #pragma unroll
         for (int o = TPR / 2; o > 0; o >>= 1)
@@ -144,27 +165,34 @@ decode8_kernel(const DecodeArgs a, uint8_t* __restrict__ scale, const Taps t) {
         }
 #pragma unroll
         for (int o = TPR; o < 32; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-        const float base = mx == -INFINITY ? 0.f : mx, cor = __expf(m - base);
-        l *= cor;
+        const float base = mx == -INFINITY ? 0.f : mx;
+        if (r0) {
+            const float cor = __expf(m - base);
+            const f32x2 cc = pair(cor, cor);
+            l *= cor;
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) acc[e] *= cor;
+            for (int e = 0; e < VEC / 2; ++e) acc[e] = mul2(acc[e], cc);
+        }
         m = mx;
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-            const float p = __expf(sc[r] - base);
+            const float p = __expf(sc[r] - base), w = p * row_scale(sb[r] >> 8);
             l += p;
-            const float w = p * scale_value(sb[r] >> 8);
-            float x[VEC];
-            v[r].get(x);
+            const f32x2 ww = pair(w, w);
+            Bytes<VEC> v;
+            v.load(&rows[warp][r][1][lane * VEC]);
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) acc[e] = fmaf(w, x[e], acc[e]);
+            for (int e = 0; e < VEC / 2; ++e) acc[e] = fma2(ww, v.get(e), acc[e]);
         }
     }
+    float out[VEC];
+#pragma unroll
+    for (int e = 0; e < VEC / 2; ++e) unpair(acc[e], out[2 * e], out[2 * e + 1]);
 #pragma unroll
     for (int o = TPR; o < 32; o <<= 1) {
         l += __shfl_xor_sync(0xffffffffu, l, o);
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) acc[e] += __shfl_xor_sync(0xffffffffu, acc[e], o);
+        for (int e = 0; e < VEC; ++e) out[e] += __shfl_xor_sync(0xffffffffu, out[e], o);
     }
     if (g == 0 && active) {
         const float inv = l == 0.f ? 0.f : (a.head_gain ? a.head_gain[h] : 1.f) / l;
@@ -172,10 +200,230 @@ decode8_kernel(const DecodeArgs a, uint8_t* __restrict__ scale, const Taps t) {
         for (int b = 0; b < VEC; b += 8) {
             float y[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) y[e] = acc[b + e] * inv;
+            for (int e = 0; e < 8; ++e) y[e] = out[b + e] * inv;
             store8(static_cast<T*>(a.out) + (size_t)sh * D + d0 + b, y);
         }
     }
+}
+
+// ---- the same step on tensor cores: bf16 queries, no scale_embed, D = 32, 64 or 128.
+//
+// Taps are the 16 rows of mma.sync (m16n8k16, f16 in, fp32 sums), the query stands in all eight columns: scores = K q without a shuffle, and after the softmax
+// O^T += V^T p without one, p turned from a result into an operand by movmatrix.  e4m3 becomes f16 exactly; the query becomes f16 after a power of two
+// that brings its largest element to [1, 2); the keys' scales multiply the scores, the values' scales the probabilities, relative to the largest scale
+// of the step.  What bounds the step is instructions, not memory: some 700 a warp instead of the 1730 of the form above, whose rows go to fp32 one by one.
+// A lane asks for the pieces of key rows g and g + 8 that it needs itself (lane (g, t): piece t); value rows go to shared memory as rows, even ones in
+// front of odd ones and pieces exchanged so that rows 2 t, 2 t + 1, 2 t + 8, 2 t + 9 are read without bank conflicts.
+template <int D> struct Mma {
+    static constexpr int KB = D >= 64 ? 16 : 8, KP = D / (4 * KB);           // bytes of a piece of a row, pieces a lane
+    static constexpr int VB = D / 8;                                         // bytes of a value row for a lane
+    static constexpr int TILES = 3, W = D == 128 ? 2 : 4;                    // 16-tap tiles a pass; warps a block
+    static constexpr int KTILE = 16 * D, STAGE = TILES * 2 * KTILE;          // key rows, then value rows
+    __device__ static __forceinline__ int value_at(int row, int byte) {
+        const int r = (row & 8) | (row & 1) << 2 | (row >> 1 & 3);
+        return r * D + (D == 128 ? byte ^ (r & 3) << 5 : D == 64 ? byte ^ (r >> 1 & 1) << 5 : byte);
+    }
+};
+__device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t f16x2(float lo, float hi) { const __half2 h = __floats2half2_rn(lo, hi); return *reinterpret_cast<const uint32_t*>(&h); }
+template <int WORDS> __device__ __forceinline__ void words_of(const void* p, uint32_t (&w)[WORDS]) {
+    if constexpr (WORDS == 4) { const uint4 v = *static_cast<const uint4*>(p); w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w; }
+    else if constexpr (WORDS == 2) { const uint2 v = *static_cast<const uint2*>(p); w[0] = v.x; w[1] = v.y; }
+    else w[0] = *static_cast<const uint32_t*>(p);
+}
+
+template <int D, bool PDL>
+__global__ void __launch_bounds__(Mma<D>::W * 32, D == 128 ? 6 : 6) decode8_mma_kernel(const DecodeArgs a, uint8_t* __restrict__ scale, const Taps t) {
+    using C = Mma<D>;
+    constexpr int TILES = C::TILES, KP = C::KP, KB = C::KB, VEC = D / 4, STEPS = D / 16, E = KB / 4;
+    if constexpr (!PDL) stream_wait();
+    __shared__ __align__(16) char smem[C::W][C::STAGE];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, tig = lane & 3;
+    const int sh = blockIdx.x * C::W + warp;                   // (sequence, head) pair
+    if (sh >= a.S * a.H) return;                               // whole warp leaves together
+    const int s = sh / a.H, h = sh - s * a.H;
+    const int head = a.head[s], fill = a.fill ? a.fill[s] : a.R;
+    uint8_t* const ring = static_cast<uint8_t*>(a.k_ring) + (size_t)sh * a.R * 2 * D;
+    uint8_t* const bytes = scale + (size_t)sh * a.R * 2;
+    char* const keys = smem[warp];
+    char* const values = smem[warp] + TILES * C::KTILE;
+
+    uint32_t qb[STEPS][2];
+    float fs = 0.f, m = -INFINITY, l = 0.f, o[STEPS][4];
+#pragma unroll
+    for (int k = 0; k < STEPS; ++k) {
+        qb[k][0] = qb[k][1] = 0u;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[k][e] = 0.f;
+    }
+    uint32_t vtop = 0u;
+#pragma unroll 1
+    for (int j0 = 0; j0 < t.J; j0 += 16 * TILES) {             // one pass for the usual tap counts
+        uint32_t sb[TILES][2];
+        bool tap[TILES][2];
+#pragma unroll
+        for (int i = 0; i < TILES; ++i)
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                const int row = g + 8 * x, j = j0 + 16 * i + row, delta = j < t.J ? t.delta(j) : 0;
+                int slot = head - delta;
+                if (slot < 0) slot += a.R;
+                tap[i][x] = j < t.J && delta < fill;
+                const bool old = tap[i][x] && delta > 0;
+                if (!old) slot = 0;
+                const uint8_t* const from = ring + (size_t)slot * (2 * D) + tig * KB;
+#pragma unroll
+                for (int k = 0; k < KP; ++k) {
+                    copy_async<KB>(keys + (((i * 2 + x) * KP + k) * 32 + lane) * KB, from + 4 * k * KB, old);
+                    copy_async<KB>(values + i * C::KTILE + C::value_at(row, (4 * k + tig) * KB), from + D + 4 * k * KB, old);
+                }
+                sb[i][x] = 127u | 127u << 8;
+                if (old) sb[i][x] = *reinterpret_cast<const uint16_t*>(bytes + 2 * slot);
+            }
+        if (j0 == 0) {
+            if constexpr (PDL) stream_wait();
+            // the query, and the new token's rows in e4m3: piece 4 k + tig of each, by every group of four lanes
+            float x[VEC], y[VEC];
+            uint32_t top = 0u;
+#pragma unroll
+            for (int k = 0; k < KP; ++k) {
+                const long long at = (long long)sh * D + (4 * k + tig) * KB;
+#pragma unroll
+                for (int b = 0; b < KB; b += 8) {
+                    const uint4 u = *reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(a.q) + at + b);
+                    qb[k * E + b / 4][0] = u.x; qb[k * E + b / 4][1] = u.y; qb[k * E + b / 4 + 1][0] = u.z; qb[k * E + b / 4 + 1][1] = u.w;
+                    float z[8];
+                    load8(static_cast<const __nv_bfloat16*>(a.k_new) + at + b, z);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) x[k * KB + b + e] = z[e];
+                    load8(static_cast<const __nv_bfloat16*>(a.v_new) + at + b, z);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) y[k * KB + b + e] = z[e];
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < STEPS; ++k)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) top = max(top, max(qb[k][e] << 16 & 0x7fff0000u, qb[k][e] & 0x7fff0000u));
+            top = group_max<4>(top);
+            int ex = (int)(top >> 23);                         // NaN and infinity stay what they are
+            ex = ex == 0 ? 127 : ex >= 254 ? 253 : ex;
+            const float down = __uint_as_float((254u - ex) << 23);
+            fs = a.scale * 1.4426950408889634f * __uint_as_float((uint32_t)ex << 23);
+#pragma unroll
+            for (int k = 0; k < STEPS; ++k)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) qb[k][e] = f16x2(__uint_as_float(qb[k][e] << 16) * down, __uint_as_float(qb[k][e] & 0xffff0000u) * down);
+            Bytes<VEC> kn, vn;
+            const uint32_t fresh = quantize<4, VEC>(x, kn) | quantize<4, VEC>(y, vn) << 8;
+            asm volatile("cp.async.wait_all;" ::: "memory");
+            if (g == 0) {
+                const bool here = t.delta(0) == 0 && tap[0][0];               // offsets ascend: only tap 0 can be delta 0
+                if (here) sb[0][0] = fresh;
+#pragma unroll
+                for (int k = 0; k < KP; ++k) {
+                    const int at = (4 * k + tig) * KB;
+                    uint8_t* const to = ring + (size_t)head * (2 * D) + at;
+#pragma unroll
+                    for (int b = 0; b < KB; b += 8) {
+                        const uint2 ku = make_uint2(kn.u[(k * KB + b) / 4], kn.u[(k * KB + b) / 4 + 1]), vu = make_uint2(vn.u[(k * KB + b) / 4], vn.u[(k * KB + b) / 4 + 1]);
+                        *reinterpret_cast<uint2*>(to + b) = ku; *reinterpret_cast<uint2*>(to + D + b) = vu;
+                        if (here) {
+                            *reinterpret_cast<uint2*>(keys + (k * 32 + lane) * KB + b) = ku;
+                            *reinterpret_cast<uint2*>(values + C::value_at(0, at) + b) = vu;
+                        }
+                    }
+                }
+                if (tig == 0) *reinterpret_cast<uint16_t*>(bytes + 2 * head) = (uint16_t)fresh;
+            }
+        } else asm volatile("cp.async.wait_all;" ::: "memory");
+        __syncwarp();
+        // ---- scores: taps g and g + 8 of a tile, the same in every column
+        float sc[TILES][2], mx = m;
+        uint32_t top = vtop;
+#pragma unroll
+        for (int i = 0; i < TILES; ++i) {
+            float c[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int k = 0; k < KP; ++k) {
+                uint32_t w[2][E];
+                words_of(keys + (((i * 2) * KP + k) * 32 + lane) * KB, w[0]);
+                words_of(keys + (((i * 2 + 1) * KP + k) * 32 + lane) * KB, w[1]);
+#pragma unroll
+                for (int e = 0; e < E; ++e) {
+                    uint32_t ka[4];
+                    e4m3x4_half2(w[0][e], ka[0], ka[2]); e4m3x4_half2(w[1][e], ka[1], ka[3]);
+                    mma(c, ka, qb[k * E + e][0], qb[k * E + e][1]);
+                }
+            }
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                const float bias = tap[i][x] ? __ldg(a.pos_bias + (j0 + 16 * i + g + 8 * x) * a.H + h) * 1.4426950408889634f : -INFINITY;
+                sc[i][x] = tap[i][x] ? fmaf(c[2 * x] * row_scale(sb[i][x] & 255u), fs, bias) : -INFINITY;
+                mx = fmaxf(mx, sc[i][x]);
+                const uint32_t vb = sb[i][x] >> 8;
+                if (tap[i][x] && vb != 255u) top = max(top, vb);
+            }
+        }
+        top = __reduce_max_sync(0xffffffffu, top);
+#pragma unroll
+        for (int b = 4; b < 32; b <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, b));
+        const float base = mx == -INFINITY ? 0.f : mx;
+        if (j0) {                                              // a later pass: what was summed so far is against the old maximum and the old scale
+            const float f = exp2f(m - base), fv = f * __uint_as_float((uint32_t)max(127 + (int)vtop - (int)top, 0) << 23);
+            l *= f;
+#pragma unroll
+            for (int k = 0; k < STEPS; ++k)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[k][e] *= fv;
+        }
+        m = mx; vtop = top;
+#pragma unroll
+        for (int i = 0; i < TILES; ++i) {
+            uint32_t pb[2];
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                const float p = exp2f(sc[i][x] - base);
+                l += p;
+                const uint32_t vb = sb[i][x] >> 8;
+                const float w = !tap[i][x] ? 0.f : p * (vb == 255u ? __uint_as_float(0x7fc00000u) : __uint_as_float((uint32_t)max(127 + (int)vb - (int)top, 0) << 23));
+                // to f16, as the operand of the product: relative 2^-11 on terms that add up
+                asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(pb[x]) : "r"(f16x2(w, w)));
+            }
+            uint32_t w[4][C::VB / 4];
+#pragma unroll
+            for (int x = 0; x < 4; ++x) words_of(values + i * C::KTILE + C::value_at(2 * tig + (x & 1) + 8 * (x >> 1), g * C::VB), w[x]);
+#pragma unroll
+            for (int e = 0; e < C::VB / 4; ++e)
+#pragma unroll
+                for (int y = 0; y < 2; ++y) {                  // values 2 y, 2 y + 1 of the word: rows g and g + 8 of m-tile 2 e + y
+                    uint32_t va[4];
+                    e4m3x4_half2(__byte_perm(w[0][e], w[1][e], y ? 0x7362 : 0x5140), va[0], va[1]);
+                    e4m3x4_half2(__byte_perm(w[2][e], w[3][e], y ? 0x7362 : 0x5140), va[2], va[3]);
+                    mma(o[2 * e + y], va, pb[0], pb[1]);
+                }
+        }
+        __syncwarp();                                          // every lane has read the rows that the next pass replaces
+    }
+#pragma unroll
+    for (int b = 4; b < 32; b <<= 1) l += __shfl_xor_sync(0xffffffffu, l, b);
+    if (tig == 0) {                                            // d = VB g + 2 (m-tile), + 1
+        const float inv = l == 0.f ? 0.f : (a.head_gain ? a.head_gain[h] : 1.f) / l * scale_value(vtop);
+        uint32_t y[STEPS];
+#pragma unroll
+        for (int k = 0; k < STEPS; ++k) y[k] = pack_bf16x2(o[k][0] * inv, o[k][2] * inv);
+        uint32_t* const to = reinterpret_cast<uint32_t*>(static_cast<__nv_bfloat16*>(a.out) + (size_t)sh * D + g * C::VB);
+#pragma unroll
+        for (int k = 0; k < STEPS; k += 2) *reinterpret_cast<uint2*>(to + k) = make_uint2(y[k], y[k + 1]);
+    }
+}
+
+template <int D> cudaError_t launch_mma(const DecodeArgs& a, uint8_t* scale, const Taps& t, cudaStream_t s, bool overlap) {
+    const unsigned blocks = (unsigned)((a.S * a.H + Mma<D>::W - 1) / Mma<D>::W);
+    return launch_after(overlap ? decode8_mma_kernel<D, true> : decode8_mma_kernel<D, false>, blocks, Mma<D>::W * 32, 0, s, a, scale, t);
 }
 
 template <typename T, int TPR, int VEC> cudaError_t launch_group(const DecodeArgs& a, uint8_t* scale, const Taps& t, cudaStream_t s, bool overlap) {
@@ -245,6 +493,11 @@ inline bool bad(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) !
 }  // namespace
 
 cudaError_t launch_decode8(const DecodeArgs& a, uint8_t* scale, const Taps& t, int dtype, cudaStream_t s, bool overlap) {
+    if (dtype == DSQG_DTYPE_BF16 && !a.scale_embed) {
+        if (a.D == 64) return launch_mma<64>(a, scale, t, s, overlap);
+        if (a.D == 32) return launch_mma<32>(a, scale, t, s, overlap);
+        if (a.D == 128) return launch_mma<128>(a, scale, t, s, overlap);
+    }
     return dtype == DSQG_DTYPE_BF16 ? launch_type<__nv_bfloat16>(a, scale, t, s, overlap) : launch_type<float>(a, scale, t, s, overlap);
 }
 

@@ -193,10 +193,14 @@ struct NormGradArgs {
     long long rows; int D; int s_dt, y_dt, x_dt;
 };
 
+// Blocks of the backward kernel that an SM holds: the grid is that many times 148, so that all of them start at once and walk the same number of rows
+// (four an SM where registers allow three took a second wave of blocks that then had a quarter of the rows to itself: 53 us instead of 44 at 65,536 x 256).
+constexpr int grad_blocks_an_sm(int W, int TPR, int V) { return TPR > 256 ? 1 : W * V >= 32 ? 1 : W * V >= 16 ? 2 : 3; }
+
 // A block walks rows a grid apart; a thread keeps the sums of its columns of dw.  The partial sums of a block's rows go to part[block],
 // added by dw_kernel: the order follows from the sizes alone.
 template <int W, int TPR, int V>
-__global__ void __launch_bounds__(TPR < kThreads ? kThreads : TPR) rms_bwd_kernel(const NormGradArgs a) {
+__global__ void __launch_bounds__(TPR < kThreads ? kThreads : TPR, grad_blocks_an_sm(W, TPR, V)) rms_bwd_kernel(const NormGradArgs a) {
     constexpr int kBlock = TPR < kThreads ? kThreads : TPR, kRows = kBlock / TPR;
     __shared__ float red[64];
     extern __shared__ float sums[];
@@ -316,24 +320,41 @@ __global__ void __launch_bounds__(kThreads) dw_part_kernel(const NormGradArgs a)
     a.part[(size_t)blockIdx.y * a.D + c] = s;
 }
 
-// dw[c] = sum over the n rows of part: 32 columns a block, its warps a 32nd of the rows each, added in warp order.
+// dw[c] = sum over the n rows of part: 32 columns a block, every 128th row a thread, all of them on their way together; added in row order of the threads.
 __global__ void __launch_bounds__(1024) dw_kernel(const float* __restrict__ part, float* __restrict__ dw, int n, int D) {
     stream_wait();
-    __shared__ float red[32][33];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
-    float s = 0.f;
-    if (c < D) {
+    __shared__ float red[128][33];
+    const int col = threadIdx.x & 7, row = threadIdx.x >> 3, c = blockIdx.x * 32 + 4 * col;
+    float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (D % 4 == 0 && c < D) {
 #pragma unroll 8
-        for (int b = warp; b < n; b += 32) s += part[(size_t)b * D + c];
+        for (int b = row; b < n; b += 128) {
+            const float4 v = __ldg(reinterpret_cast<const float4*>(part + (size_t)b * D + c));
+            s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
+        }
+    } else {
+        for (int b = row; b < n; b += 128) {
+            const float* p = part + (size_t)b * D + c;
+            if (c < D) s.x += p[0];
+            if (c + 1 < D) s.y += p[1];
+            if (c + 2 < D) s.z += p[2];
+            if (c + 3 < D) s.w += p[3];
+        }
     }
-    red[warp][lane] = s;
+    red[row][4 * col] = s.x; red[row][4 * col + 1] = s.y; red[row][4 * col + 2] = s.z; red[row][4 * col + 3] = s.w;
     __syncthreads();
-    if (warp == 0 && c < D) {
-        s = 0.f;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    float t = 0.f;
 #pragma unroll
-        for (int w = 0; w < 32; ++w) s += red[w][lane];
-        dw[c] = s;
-    }
+    for (int i = 0; i < 4; ++i) t += red[warp * 4 + i][lane];
+    __syncthreads();
+    red[warp][lane] = t;
+    __syncthreads();
+    if (warp) return;
+    t = 0.f;
+#pragma unroll
+    for (int w = 0; w < 32; ++w) t += red[w][lane];
+    if (blockIdx.x * 32 + lane < D) dw[blockIdx.x * 32 + lane] = t;
 }
 
 inline bool bad(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) != 0; }
@@ -363,8 +384,15 @@ inline int rows_per_block(Shape s) {
 }
 // Blocks of the backward kernel, which follow from the sizes alone.
 inline int grad_blocks(long long rows, Shape s) {
+    int an_sm = 3;
+    switch (s) {
+        case k8x32x2: case k8x256x2: case k1x256x16: an_sm = 2; break;
+        case k8x32x4: case k8x256x4: case k8x1024x4: an_sm = 1; break;
+        case kWide: an_sm = 4; break;
+        default: break;
+    }
     const long long b = (rows + rows_per_block(s) - 1) / rows_per_block(s);
-    return (int)(b < 148 * 4 ? b : 148 * 4);
+    return (int)(b < 148 * an_sm ? b : 148 * an_sm);
 }
 
 }  // namespace

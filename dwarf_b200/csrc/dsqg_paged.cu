@@ -15,85 +15,143 @@ struct MoveArgs {
     PageArgs c;
     const int32_t* cu; const int32_t* start;
     void* k; void* v;
-    long long tokens, k_token, k_head, v_token, v_head;        // element strides
-    int dtype;
+    long long k_token, k_head, v_token, v_head;                // element strides
+    int tokens, dtype;
 };
 
-// (sequence, position) of token t, or s = -1: a row in front of the first sequence or behind the last.
-__device__ __forceinline__ int sequence_of(const MoveArgs& a, long long t, long long& position) {
-    int lo = 0, hi = a.c.S;
-    if (t < __ldg(a.cu) || t >= __ldg(a.cu + hi)) return -1;
-    while (hi - lo > 1) {                                       // cu[lo] <= t < cu[hi]
-        const int mid = (lo + hi) >> 1;
-        if (__ldg(a.cu + mid) <= t) lo = mid; else hi = mid;
+// (sequence, position) of token t, or s = -1: a row in front of the first sequence or behind the last.  All lanes of a warp take part, LPR of them with the same
+// token.  Up to 32 sequences a lane looks at one boundary and the warp counts those at or below its tokens: one load to wait for instead of five.
+template <int LPR> __device__ __forceinline__ int sequence_of(const MoveArgs& a, int t, bool there, long long& position) {
+    const int S = a.c.S, lane = threadIdx.x & 31;
+    int s = -1, from = 0;
+    if (S <= 32) {
+        const int first = __ldg(a.cu), edge = __ldg(a.cu + 1 + min(lane, S - 1));
+        int count = 0;
+#pragma unroll
+        for (int q = 0; q < 32 / LPR; ++q) {
+            const int other = __shfl_sync(0xffffffffu, t, q * LPR);
+            const unsigned below = __ballot_sync(0xffffffffu, lane < S && edge <= other);
+            if (lane / LPR == q) count = __popc(below);
+        }
+        from = __shfl_sync(0xffffffffu, edge, max(count - 1, 0));
+        if (count == 0) from = first;
+        if (there && t >= first && count < S) s = count;
+    } else if (there) {
+        int lo = 0, hi = S;
+        if (t >= __ldg(a.cu) && t < __ldg(a.cu + hi)) {
+            while (hi - lo > 1) {                               // cu[lo] <= t < cu[hi]
+                const int mid = (lo + hi) >> 1;
+                if (__ldg(a.cu + mid) <= t) lo = mid; else hi = mid;
+            }
+            s = lo; from = __ldg(a.cu + lo);
+        }
     }
-    position = t - __ldg(a.cu + lo) + (a.start ? __ldg(a.start + lo) : 0);
-    return lo;
+    if (s >= 0) position = (long long)t - from + (a.start ? __ldg(a.start + s) : 0);
+    return s;
 }
 
-template <int LPR, bool WRITE>
+// Eight elements as they lie in memory, so that the rows of all heads are asked for before one is used.
+struct Raw8 {
+    uint4 a, b;
+    __device__ __forceinline__ void load(const void* p, long long i, int dtype) {
+        if (dtype == DSQG_DTYPE_F32) { const uint4* s = reinterpret_cast<const uint4*>(static_cast<const float*>(p) + i); a = __ldg(s); b = __ldg(s + 1); }
+        else if (dtype == DSQG_DTYPE_BF16) a = __ldg(reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(p) + i));
+        else { const uint2 u = *reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(p) + i); a.x = u.x; a.y = u.y; }
+    }
+    __device__ __forceinline__ void get(float (&x)[8], int dtype) const {
+        if (dtype == DSQG_DTYPE_F32) {
+            const uint32_t u[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = __uint_as_float(u[e]);
+        } else if (dtype == DSQG_DTYPE_BF16) {
+            const uint32_t u[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) { x[2 * e] = __uint_as_float(u[e] << 16); x[2 * e + 1] = __uint_as_float(u[e] & 0xffff0000u); }
+        } else { e4m3x4_float(a.x, x); e4m3x4_float(a.y, x + 4); }
+    }
+};
+
+// HC heads of a token a group of lanes: where the token goes is found once for them, and their rows are on their way together (8 tokens of up to 2048
+// positions, 12 heads of 64 into 8 bits, one head a group: 12.5 us, most of it 64-bit divisions; 32-bit ones 11.4).
+template <int LPR, int HC, bool WRITE>
 __global__ void __launch_bounds__(kT) move_kernel(const MoveArgs a) {
     stream_wait();
-    const long long pair = ((long long)blockIdx.x * kT + threadIdx.x) / LPR;
+    const unsigned group = blockIdx.x * (kT / LPR) + threadIdx.x / LPR, per = (a.c.H + HC - 1) / HC;
     const int d = (threadIdx.x % LPR) * 8, D = a.c.D;
-    const long long t = pair / a.c.H;
-    const int h = (int)(pair - t * a.c.H);
-    const bool there = t < a.tokens, on = there && d < D;
-    long long position = 0, slot = -1;
-    int s = there ? sequence_of(a, t, position) : -1;
-    if (s >= 0 && position >= 0 && position < (long long)a.c.columns * a.c.page) {
-        const long long first = a.c.rows_of(s, h, (int)(position / a.c.page));
-        if (first >= 0) slot = (first + position % a.c.page) * 2;
+    const int t = (int)(group / per), h0 = (int)(group - (unsigned)t * per) * HC;
+    const bool there = t < a.tokens, on = there && d < D, f8 = a.c.dtype == DSQG_DTYPE_E4M3;
+    const long long ki = (long long)t * a.k_token + h0 * a.k_head + d, vi = (long long)t * a.v_token + h0 * a.v_head + d, step = 2LL * a.c.page;
+    Raw8 k[HC], v[HC];
+#pragma unroll
+    for (int i = 0; i < HC; ++i) {                             // what is written does not wait for where it goes
+        k[i].a = k[i].b = v[i].a = v[i].b = make_uint4(0u, 0u, 0u, 0u);
+        if (WRITE && h0 + i < a.c.H && on) { k[i].load(a.k, ki + i * a.k_head, a.dtype); v[i].load(a.v, vi + i * a.v_head, a.dtype); }
     }
-    const bool f8 = a.c.dtype == DSQG_DTYPE_E4M3;
-    const long long ki = t * a.k_token + h * a.k_head + d, vi = t * a.v_token + h * a.v_head + d;
-    float k[8] = {0, 0, 0, 0, 0, 0, 0, 0}, v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-    if constexpr (WRITE) {
-        if (on && slot >= 0) { load8_as(a.k, ki, a.dtype, k); load8_as(a.v, vi, a.dtype, v); }
-        if (f8) {
-            uint32_t kt = 0u, vt = 0u;
+    long long position = 0, slot = -1;
+    const int s = sequence_of<LPR>(a, t, there, position);
+    if (s >= 0 && position >= 0 && position < (long long)a.c.columns * a.c.page) {
+        const unsigned at = (unsigned)position, column = at / (unsigned)a.c.page;
+        const long long first = a.c.rows_of(s, h0, (int)column);
+        if (first >= 0) slot = (first + (at - column * a.c.page)) * 2;
+    }
+    uint32_t sb[HC];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) { kt = max(kt, abs_bits(k[e])); vt = max(vt, abs_bits(v[e])); }
-            const uint32_t kb = row_scale_byte(group_max<LPR>(kt)), vb = row_scale_byte(group_max<LPR>(vt));
-            const float ik = scale_inverse(kb), iv = scale_inverse(vb);
+    for (int i = 0; i < HC; ++i) {
+        sb[i] = 127u | 127u << 8;
+        if (!WRITE && h0 + i < a.c.H && on && slot >= 0) {
+            const long long at = slot + i * step;
+            k[i].load(a.c.kv, at * D + d, a.c.dtype); v[i].load(a.c.kv, (at + 1) * D + d, a.c.dtype);
+            if (f8) sb[i] = *reinterpret_cast<const uint16_t*>(a.c.scale + at);
+        }
+    }
 #pragma unroll
-            for (int e = 0; e < 8; ++e) { k[e] *= ik; v[e] *= iv; }
-            if (d == 0 && slot >= 0) *reinterpret_cast<uint16_t*>(a.c.scale + slot) = (uint16_t)(kb | vb << 8);
-        }
-        if (on && slot >= 0) {
-            store8_as(a.c.kv, slot * D + d, a.c.dtype, k);
-            store8_as(a.c.kv, (slot + 1) * D + d, a.c.dtype, v);
-        }
-    } else if (on) {
-        if (slot >= 0) {
-            load8_as(a.c.kv, slot * D + d, a.c.dtype, k);
-            load8_as(a.c.kv, (slot + 1) * D + d, a.c.dtype, v);
+    for (int i = 0; i < HC; ++i) {
+        float x[8], y[8];
+        const long long at = slot + i * step;
+        const bool mine = h0 + i < a.c.H && on;
+        if constexpr (WRITE) {
+            k[i].get(x, a.dtype); v[i].get(y, a.dtype);
             if (f8) {
-                const uint32_t b = *reinterpret_cast<const uint16_t*>(a.c.scale + slot);
-                const float sk = scale_value(b & 255u), sv = scale_value(b >> 8);
+                uint32_t kt = 0u, vt = 0u;
 #pragma unroll
-                for (int e = 0; e < 8; ++e) { k[e] *= sk; v[e] *= sv; }
+                for (int e = 0; e < 8; ++e) { kt = max(kt, abs_bits(x[e])); vt = max(vt, abs_bits(y[e])); }
+                const uint32_t kb = row_scale_byte(group_max<LPR>(kt)), vb = row_scale_byte(group_max<LPR>(vt));
+                const float ik = scale_inverse(kb), iv = scale_inverse(vb);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) { x[e] *= ik; y[e] *= iv; }
+                if (d == 0 && mine && slot >= 0) *reinterpret_cast<uint16_t*>(a.c.scale + at) = (uint16_t)(kb | vb << 8);
             }
-        } else if (s >= 0) {
+            if (mine && slot >= 0) {
+                store8_as(a.c.kv, at * D + d, a.c.dtype, x);
+                store8_as(a.c.kv, (at + 1) * D + d, a.c.dtype, y);
+            }
+        } else if (mine) {
+            k[i].get(x, a.c.dtype); v[i].get(y, a.c.dtype);
+            // a position that the table has no page for is NaN, a row of no sequence (whose bytes are zeros) zeros
+            const float nan = __uint_as_float(0x7fc00000u), sk = s >= 0 && slot < 0 ? nan : f8 ? scale_value(sb[i] & 255u) : 1.f, sv = s >= 0 && slot < 0 ? nan : f8 ? scale_value(sb[i] >> 8) : 1.f;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) k[e] = v[e] = __uint_as_float(0x7fc00000u);      // a position the table has no page for
+            for (int e = 0; e < 8; ++e) { x[e] *= sk; y[e] *= sv; }
+            store8_as(a.k, ki + i * a.k_head, a.dtype, x);
+            store8_as(a.v, vi + i * a.v_head, a.dtype, y);
         }
-        store8_as(a.k, ki, a.dtype, k);
-        store8_as(a.v, vi, a.dtype, v);
     }
 }
 
-template <bool WRITE> cudaError_t launch_move(const MoveArgs& a, cudaStream_t s) {
+template <bool WRITE, int HC> cudaError_t launch_move(const MoveArgs& a, cudaStream_t s) {
     const int lanes = a.c.D / 8, lpr = lanes <= 1 ? 1 : lanes <= 2 ? 2 : lanes <= 4 ? 4 : lanes <= 8 ? 8 : 16;
-    const long long threads = a.tokens * a.c.H * lpr;
-    const unsigned blocks = (unsigned)((threads + kT - 1) / kT);
+    const unsigned blocks = (unsigned)(((long long)a.tokens * ((a.c.H + HC - 1) / HC) * lpr + kT - 1) / kT);
     switch (lpr) {
-        case 1: return launch_after(move_kernel<1, WRITE>, blocks, kT, 0, s, a);
-        case 2: return launch_after(move_kernel<2, WRITE>, blocks, kT, 0, s, a);
-        case 4: return launch_after(move_kernel<4, WRITE>, blocks, kT, 0, s, a);
-        case 8: return launch_after(move_kernel<8, WRITE>, blocks, kT, 0, s, a);
-        default: return launch_after(move_kernel<16, WRITE>, blocks, kT, 0, s, a);
+        case 1: return launch_after(move_kernel<1, HC, WRITE>, blocks, kT, 0, s, a);
+        case 2: return launch_after(move_kernel<2, HC, WRITE>, blocks, kT, 0, s, a);
+        case 4: return launch_after(move_kernel<4, HC, WRITE>, blocks, kT, 0, s, a);
+        case 8: return launch_after(move_kernel<8, HC, WRITE>, blocks, kT, 0, s, a);
+        default: return launch_after(move_kernel<16, HC, WRITE>, blocks, kT, 0, s, a);
     }
+}
+// Heads a group: three where they divide up evenly, two otherwise (us, write and read back of 6820 tokens, 12 heads of 64, 8 bits: one 11.4 and 8.9, two 10.6 and
+// 8.2, three 10.0 and 7.7, four 12.5 and 9.6; read of 7800 tokens, 8 heads of 128: two 22.5, three 24.3, four 25.5).
+template <bool WRITE> cudaError_t launch_move_heads(const MoveArgs& a, cudaStream_t s) {
+    return a.c.H == 1 ? launch_move<WRITE, 1>(a, s) : a.c.H % 3 == 0 ? launch_move<WRITE, 3>(a, s) : launch_move<WRITE, 2>(a, s);
 }
 
 // ---- attention of one new token, CUDA cores: fp32 arithmetic for any types, D a multiple of 8 up to 128, pages of any length.
@@ -294,9 +352,9 @@ int move_args(const dsqg_pages* c, const int32_t* cu, const int32_t* start, void
     if (!cu || !k || !v) return DSQG_ERR_NULL_POINTER;
     if (int rc = page_args(c, &a->c)) return rc;
     if (dtype != DSQG_DTYPE_BF16 && dtype != DSQG_DTYPE_F32) return DSQG_ERR_BAD_DTYPE;
-    if (tokens < 1 || tokens > 0x7fffffffLL || tokens * c->heads * 16 > 0x7fffffffLL * kT) return DSQG_ERR_BAD_SHAPE;
+    if (tokens < 1 || tokens > 0x7fffffffLL / c->heads - kT) return DSQG_ERR_BAD_SHAPE;
     if (bad(k) || bad(v) || k_token % 8 || k_head % 8 || v_token % 8 || v_head % 8) return DSQG_ERR_MISALIGNED;
-    a->cu = cu; a->start = start; a->k = k; a->v = v; a->tokens = tokens; a->dtype = dtype;
+    a->cu = cu; a->start = start; a->k = k; a->v = v; a->tokens = (int)tokens; a->dtype = dtype;
     a->k_token = k_token; a->k_head = k_head; a->v_token = v_token; a->v_head = v_head;
     return DSQG_OK;
 }
@@ -312,14 +370,14 @@ int dsqg_paged_write(const dsqg_pages* cache, const void* k, const void* v, long
                      const int32_t* cu_seqlens, const int32_t* start, long long tokens, int dtype, void* stream) {
     MoveArgs a;
     if (int rc = move_args(cache, cu_seqlens, start, const_cast<void*>(k), const_cast<void*>(v), k_token, k_head, v_token, v_head, tokens, dtype, &a)) return rc;
-    return status(launch_move<true>(a, static_cast<cudaStream_t>(stream)));
+    return status(launch_move_heads<true>(a, static_cast<cudaStream_t>(stream)));
 }
 
 int dsqg_paged_read(const dsqg_pages* cache, void* k, void* v, const int32_t* cu_seqlens, const int32_t* start, long long tokens, int dtype, void* stream) {
     MoveArgs a;
     const long long D = cache ? cache->D : 0, HD = cache ? D * cache->heads : 0;
     if (int rc = move_args(cache, cu_seqlens, start, k, v, HD, D, HD, D, tokens, dtype, &a)) return rc;
-    return status(launch_move<false>(a, static_cast<cudaStream_t>(stream)));
+    return status(launch_move_heads<false>(a, static_cast<cudaStream_t>(stream)));
 }
 
 size_t dsqg_paged_step_scratch_bytes(int sequences, int heads, int q_heads, int D, int max_length) {

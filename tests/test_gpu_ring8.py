@@ -20,8 +20,10 @@ def rings(S, H, R, D, g):
     return v.float().to(E4).to(DEV), byte.view(torch.float8_e8m0fnu).to(DEV)
 
 
-def oracle(q, kn, vn, kv, ks, head, fill, pb, gain, se, offsets):
-    """(out, bound): the step in 64 bits on what the ring holds after it, and what may be off before the result is rounded."""
+def oracle(q, kn, vn, kv, ks, head, fill, pb, gain, se, offsets, f16):
+    """(out, bound): the step in 64 bits on what the ring holds after it, and what may be off before the result is rounded.  f16: probabilities
+    are operands in f16 (relative 2^-11 each, and values below its normal range are off by at most 2^-25 of the largest value a tap), and the query is after
+    a power of two that brings its largest element to [1, 2) (elements off by at most 2^-25 of that)."""
     S, H, R, _, D = kv.shape
     rows = dequantize64(kv, ks)
     out, bound = torch.zeros(S, H, D, dtype=torch.float64), torch.zeros(S, H, D, dtype=torch.float64)
@@ -36,7 +38,11 @@ def oracle(q, kn, vn, kv, ks, head, fill, pb, gain, se, offsets):
                 k = k + se[[j for j, _ in taps]]
             o, spread, ds = attention64(q[s, h][None], k, v, 1 / math.sqrt(D), pb[[j for j, _ in taps], h])
             out[s, h] = o[0] * gain[h]
-            bound[s, h] = (2 * ds[0] + 64 * 2.0 ** -24) * spread[0] * gain[h].abs()
+            bound[s, h] = (2 * ds[0] + 64 * 2.0 ** -24) * spread[0]
+            if f16:
+                bound[s, h] += 2.0 ** -11 * spread[0] + len(at) * 2.0 ** -25 * v.abs().max()
+                bound[s, h] += 2 * (2.0 ** -24 * q[s, h].abs().max() * k.abs().sum(1).max() / math.sqrt(D)) * spread[0]
+            bound[s, h] *= gain[h].abs()
     return out, bound
 
 
@@ -70,7 +76,8 @@ def test_step(S, H, D, name, dt, overlap):
         for s in range(S):
             want[s, :, head[s]], want_s[s, :, head[s]] = new[s], new_s[s]
         assert torch.equal(got, want) and torch.equal(got_s, want_s)              # the new slot, bit for bit, and no other
-        o, b = oracle(q.double(), kn, vn, kv1, ks1, head.tolist(), fill.tolist(), pb.double(), gain.double(), None if se is None else se.double(), offsets)
+        o, b = oracle(q.double(), kn, vn, kv1, ks1, head.tolist(), fill.tolist(), pb.double(), gain.double(), None if se is None else se.double(), offsets,
+                      dt is torch.bfloat16 and se is None and D in (32, 64, 128))
         err = (out.double().cpu() - o).abs()
         assert out.dtype is dt and (err <= HALF[dt] * o.abs() + b * (1 + HALF[dt])).all(), (err - HALF[dt] * o.abs() - b).max()
 
