@@ -13,8 +13,9 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
+from .int4 import Int4Linear, Rows8
 from .modules import DSQGAttentionN_Fused, DSQGAttentionQW
-from .ops import OFFSETS_43
+from .ops import OFFSETS_43, rms_norm, rms_norm_e4m3
 
 
 class RMSNorm(nn.Module):
@@ -25,6 +26,15 @@ class RMSNorm(nn.Module):
 
     def forward(self, x):
         return F.rms_norm(x, (x.shape[-1],), self.weight, self.eps)
+
+    def add(self, branch, stream, rows8=False, out_dtype=None):
+        """(norm(stream + branch), stream + branch) in one pass (`rms_norm`; branch None: nothing is added); rows8: the norm in 8 bits as Rows8."""
+        x, residual = (stream, None) if branch is None else (branch, stream)
+        if rows8:
+            y = rms_norm_e4m3(x, self.weight, residual, self.eps)
+            return Rows8(y[0], y[1]), stream if branch is None else y[2]
+        y = rms_norm(x, self.weight, residual, self.eps, out_dtype)
+        return (y, stream) if branch is None else y
 
 
 class FFN(nn.Module):
@@ -54,6 +64,13 @@ class FullCausalAttention(nn.Module):
 
     def forward(self, x):
         return self.attend(x)[0]
+
+    def decode_paged(self, x, cache, layer):
+        """x [S,D] (or Rows8 for 4-bit projections): one new token per sequence against layer `layer` of a PagedKVCache."""
+        qkv = self.qkv_proj(x)
+        S, D = qkv.shape[0], qkv.shape[1] // 3
+        q, k, v = (u.view(S, self.heads, D // self.heads).to(cache.step_dtype) for u in qkv.split(D, -1))
+        return self.out_proj(cache.step(layer, q, k, v).reshape(S, D).to(qkv.dtype))
 
     def decode(self, x, k_cache, v_cache, t):
         """x [S,D]: token at position t; k_cache, v_cache [S,H,T,HD] hold positions < t and
@@ -86,13 +103,17 @@ class Block(nn.Module):
 
 
 class CondMLM(nn.Module):
-    """attention = "condM": DSQG layers with the position bias only (the reference's condM,
+    """fused_norms=True runs every norm together with the addition in front of it (`rms_norm`, one pass forward and one backward) instead of
+    F.rms_norm and a separate sum; under bf16 autocast the norm then leaves in bf16, which is what the projections behind it read.
+
+    attention = "condM": DSQG layers with the position bias only (the reference's condM,
     kernels/dsqg_attention_v2.py:434-477) -- the shape the end-to-end benchmark configuration names;
     "condU": with scale_embed and the per-head gain (train/train_2048_condU.py:116-205)."""
 
     def __init__(self, vocab=32000, dim=256, heads=8, layers=6, ffn=1024, seq_len=2048,
-                 full_attention_layer=5, offsets=OFFSETS_43, attention="condM"):
+                 full_attention_layer=5, offsets=OFFSETS_43, attention="condM", fused_norms=False):
         super().__init__()
+        self.fused_norms = fused_norms
         self.embedding = nn.Embedding(vocab, dim)
         self.pos_embed = nn.Embedding(seq_len, dim)
         self.blocks = nn.ModuleList(Block(dim, heads, ffn, seq_len, i == full_attention_layer, offsets, attention)
@@ -110,9 +131,33 @@ class CondMLM(nn.Module):
     def forward(self, ids):
         B, N = ids.shape
         x = self.embedding(ids) + self.pos_embed(torch.arange(N, device=ids.device))[None]
+        if self.fused_norms:
+            half = torch.bfloat16 if torch.is_autocast_enabled("cuda") and torch.get_autocast_dtype("cuda") == torch.bfloat16 else None
+            branch = None
+            for blk in self.blocks:
+                y, x = blk.norm1.add(branch, x, out_dtype=half)
+                y, x = blk.norm2.add(blk.attn(y), x, out_dtype=half)
+                branch = blk.ffn(y)
+            return F.linear(self.norm.add(branch, x, out_dtype=half)[0], self.embedding.weight)
         for blk in self.blocks:
             x = blk(x)
         return F.linear(self.norm(x), self.embedding.weight)       # tied lm_head
+
+    def quantize_weights(self, group=None):
+        """Every projection of the blocks in 4 bits (`Int4Linear`, in place, inference only; embeddings and the tied lm_head stay as they are).  group:
+        32, 64 or 128 columns a scale, default the largest of them that divides the projection's input width."""
+        def convert(linear):
+            n = linear.in_features
+            g = group or next((g for g in (128, 64, 32) if n % g == 0), None)
+            if g is None:
+                raise ValueError(f"quantize_weights: an input width of {n} is no multiple of 32")
+            return Int4Linear.from_linear(linear, g)
+        for blk in self.blocks:
+            for m in (blk.attn, blk.ffn):
+                for name, child in list(m.named_children()):
+                    if type(child) is nn.Linear:
+                        setattr(m, name, convert(child))
+        return self
 
     # ---- incremental decoding over the O(1) DSQG rings -------------------------------------
     # The reference's generate() re-runs the model on the whole prefix for every new token
@@ -120,22 +165,37 @@ class CondMLM(nn.Module):
     # a DSQG layer needs the last max(offset)+1 keys/values, the one full-attention layer keeps all.
 
     @torch.no_grad()
-    def prefill(self, ids, max_len=None):
+    def prefill(self, ids, max_len=None, cache_dtype=None, page_size=64):
         """Runs the prompt ids [S,N] through the model, fills the decode caches from the k, v every
-        layer computed and returns (logits of the last position [S,vocab], state)."""
+        layer computed and returns (logits of the last position [S,vocab], state).
+
+        cache_dtype (bf16 or float8_e4m3fn) keeps the full-attention layers in a PagedKVCache of that type and the DSQG rings likewise, and has
+        decode_token run its norms fused with the additions in front of them, in 8 bits where 4-bit projections (`quantize_weights`) read them; the
+        default keeps a contiguous cache of max_len positions in the model's type and bf16 rings."""
         from .decode import DSQGRingCache
+        from .paged import PagedKVCache
         S, N = ids.shape
         max_len = self.pos_embed.num_embeddings if max_len is None else max_len
         dsqg_blocks = [i for i, b in enumerate(self.blocks) if not isinstance(b.attn, FullCausalAttention)]
         first = self.blocks[dsqg_blocks[0]].attn
         cache = DSQGRingCache(len(dsqg_blocks), S, first.num_heads, first.head_dim, first._offsets,
-                              dtype=torch.bfloat16, device=ids.device)
+                              dtype=cache_dtype or torch.bfloat16, device=ids.device)
         state = {"cache": cache, "ring_of": {b: i for i, b in enumerate(dsqg_blocks)}, "t": N, "full": {}}
+        full_blocks = [i for i in range(len(self.blocks)) if i not in state["ring_of"]]
+        if cache_dtype is not None:
+            state["paged"], state["page_of"] = None, {b: i for i, b in enumerate(full_blocks)}
+            if full_blocks:
+                full = self.blocks[full_blocks[0]].attn
+                state["paged"] = PagedKVCache(len(full_blocks), S, full.heads, self.embedding.embedding_dim // full.heads, max_len, page_size=page_size,
+                                              dtype=cache_dtype, device=ids.device)
+                chunk = state["paged"].extend([N] * S)
         x = self.embedding(ids) + self.pos_embed(torch.arange(N, device=ids.device))[None]
         for i, blk in enumerate(self.blocks):
             x, k, v = blk.forward_kv(x)
             if i in state["ring_of"]:
                 cache.prefill(state["ring_of"][i], k, v)
+            elif cache_dtype is not None:
+                state["paged"].write(state["page_of"][i], *(u.transpose(1, 2).reshape(S * N, u.shape[1], u.shape[3]) for u in (k, v)), chunk)
             else:
                 kc = torch.zeros(S, k.shape[1], max_len, k.shape[3], dtype=k.dtype, device=k.device)
                 vc = torch.zeros_like(kc)
@@ -152,6 +212,8 @@ class CondMLM(nn.Module):
             raise ValueError("decode_token: position beyond the model's seq_len")
         cache = state["cache"]
         cache.advance()
+        if "paged" in state:
+            return self._decode_serving(ids_t, state)
         x = self.embedding(ids_t) + self.pos_embed.weight[t]
         for i, blk in enumerate(self.blocks):
             h = blk.norm1(x)
@@ -165,11 +227,26 @@ class CondMLM(nn.Module):
         state["t"] = t + 1
         return F.linear(self.norm(x), self.embedding.weight)
 
+    def _decode_serving(self, ids_t, state):
+        t, cache, pages = state["t"], state["cache"], state["paged"]
+        if pages is not None:
+            pages.advance()
+        x, branch = self.embedding(ids_t) + self.pos_embed.weight[t], None
+        for i, blk in enumerate(self.blocks):
+            full = i not in state["ring_of"]
+            reads = (blk.attn.qkv_proj,) if full else (blk.attn.qkv_proj, blk.attn.gate_proj)
+            h, x = blk.norm1.add(branch, x, rows8=all(type(p) is Int4Linear for p in reads))
+            branch = blk.attn.decode_paged(h, pages, state["page_of"][i]) if full else blk.attn.decode(h, cache, state["ring_of"][i], overlap=True)
+            h, x = blk.norm2.add(branch, x, rows8=type(blk.ffn.fc1) is Int4Linear)
+            branch = blk.ffn(h)
+        state["t"] = t + 1
+        return F.linear(self.norm.add(branch, x)[0], self.embedding.weight)
+
     @torch.no_grad()
-    def generate(self, ids, max_new_tokens, temperature=0.0, generator=None):
+    def generate(self, ids, max_new_tokens, temperature=0.0, generator=None, cache_dtype=None):
         """Greedy (temperature 0) or sampled continuation of ids [S,N]: one prefill, then one
-        decode_token per new token.  Returns [S, N + max_new_tokens]."""
-        logits, state = self.prefill(ids, max_len=ids.shape[1] + max_new_tokens)
+        decode_token per new token.  Returns [S, N + max_new_tokens].  cache_dtype: as in prefill."""
+        logits, state = self.prefill(ids, max_len=ids.shape[1] + max_new_tokens, cache_dtype=cache_dtype)
         out = [ids]
         for step in range(max_new_tokens):
             if temperature > 0:

@@ -168,16 +168,17 @@ class _DSQGAttentionBase(nn.Module):
         return self.attend(x, kv_inject)[0] if y is None else self.dropout(y)
 
     def decode(self, x, cache, layer, overlap=False):
-        """One new token per sequence: x [S,D] -> [S,D], reading the previous tokens' k, v from
+        """One new token per sequence: x [S,D] (Rows8 where qkv_proj and gate_proj are Int4Linear) -> [S,D], reading the previous tokens' k, v from
         ring `layer` of `cache` (a DSQGRingCache whose `advance()` ran for this token) and storing
         this token's there.  The reference has no such path: its generate() re-runs the whole
         prefix (train/train_2048_condU.py:463-487)."""
-        S, D = x.shape
+        qkv = self.qkv_proj(x)                                  # x may be Rows8 where the projections take it
+        S, D = qkv.shape[0], self.embedding_dim
         H, HD = self.num_heads, self.head_dim
-        q, k, v = (t.reshape(S, H, HD).to(cache.k.dtype).contiguous() for t in self.qkv_proj(x).split(D, dim=-1))
+        q, k, v = (t.reshape(S, H, HD).to(getattr(cache, "step_dtype", cache.k.dtype)).contiguous() for t in qkv.split(D, dim=-1))
         out = cache.step(layer, q, k, v, self.pos_bias, getattr(self, "if_gain", None),
                          getattr(self, "scale_embed", None), overlap=overlap)
-        flat = out.reshape(S, D).to(x.dtype)
+        flat = out.reshape(S, D).to(qkv.dtype if isinstance(x, tuple) else x.dtype)
         return self.out_proj(flat * torch.sigmoid(self.gate_proj(x)))
 
     def attn_summary(self):
