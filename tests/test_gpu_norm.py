@@ -71,6 +71,13 @@ def test_forward_and_gradients(shape, x_dt, s_dt, y_dt):
     assert grads[1].dtype is w.dtype and grads[0].dtype is x_dt
 
 
+# More rows than a block for each takes, of widths that are and are not a multiple of eight: a block's sums of columns go over rows a grid apart.
+@pytest.mark.parametrize("shape", [(25000, 7), (12001, 40), (7000, 65), (6001, 201), (1999, 1111), (1601, 2048), (700, 4097), (601, 8192), (301, 16383), (300, 30001)], ids=str)
+@pytest.mark.parametrize("x_dt,s_dt,y_dt", [(BF, BF, BF), (BF, F, BF), (F, F, F)])
+def test_many_rows(shape, x_dt, s_dt, y_dt):
+    test_forward_and_gradients(shape, x_dt, s_dt, y_dt)
+
+
 def test_gradients_are_the_differences_of_the_formula():
     x, r, w, g = make((3, 24), F, F, seed=3)
     dy, dh = torch.randn(3, 24, generator=g).double(), torch.randn(3, 24, generator=g).double()
