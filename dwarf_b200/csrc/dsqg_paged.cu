@@ -256,51 +256,77 @@ __global__ void __launch_bounds__(kStepThreads) step_kernel(const StepArgs a) {
     }
 }
 
-// Joins the parts of a sequence: one block per (sequence, query head), its warps every eighth part, added in warp order.  (One warp per row, parts one
-// after the other: 40 us for 128 rows of 98 parts, which is a chain of loads.)
+// Joins the parts of a sequence: W warps per (sequence, query head), four parts a warp at a time (maximum, sum and values asked for together), the warps
+// added in order.  What it waits for is memory: W so that no warp goes round twice up to 32 parts, and not more, for there may be many rows of few parts.
+// (One warp per row, parts one after the other: 40 us for 128 rows of 98 parts, which is a chain of loads.)
 constexpr int kJoinWarps = 8;
-__global__ void __launch_bounds__(kJoinWarps * 32) join_kernel(const StepArgs a) {
+template <int W> __global__ void __launch_bounds__(kJoinWarps * 32) join_kernel(const StepArgs a) {
+    constexpr int kParts = 4;
     __shared__ float4 sums[kJoinWarps][32];
-    __shared__ float sl[kJoinWarps];
+    __shared__ float2 tops[kJoinWarps];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, D = a.c.D, d = 4 * lane, sub = warp % W, rows = a.c.S * a.c.H * a.G;
+    const int row = blockIdx.x * (kJoinWarps / W) + warp / W;
+    // The length is read before the wait: this kernel starts when every block of the one in front of it has waited for all that came before.
+    int n = 0;
+    if (row < rows) {
+        const Range r = range_of(a, row / (a.c.H * a.G), 0);
+        n = r.length ? (r.length + a.chunk - 1) / a.chunk : 1;
+    }
     stream_wait();
-    const int row = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, D = a.c.D, d = 4 * lane;
-    const int s = row / (a.c.H * a.G);
-    const Range r = range_of(a, s, 0);
-    const int n = r.length ? (r.length + a.chunk - 1) / a.chunk : 1;
     const float2* ml = a.ml + (long long)row * a.parts;
     const float* acc = a.acc + (long long)row * a.parts * D;
-    float M = -INFINITY;
-    for (int p = lane; p < n; p += 32) M = fmaxf(M, ml[p].x);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-    const float base = M == -INFINITY ? 0.f : M;
-    float L = 0.f;
+    float M = -INFINITY, L = 0.f;
     float4 A = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-    for (int p = warp; p < n; p += kJoinWarps) {
-        const float2 v = ml[p];
-        const float4 x = d < D ? *reinterpret_cast<const float4*>(acc + (long long)p * D + d) : A;
+    const auto add = [&](const float2 v, const float4 x, float base) {
         const float w = exp2f(v.x - base);
         L = fmaf(w, v.y, L);
         A.x = fmaf(w, x.x, A.x); A.y = fmaf(w, x.y, A.y); A.z = fmaf(w, x.z, A.z); A.w = fmaf(w, x.w, A.w);
-    }
-    sums[warp][lane] = A;
-    if (lane == 0) sl[warp] = L;
-    __syncthreads();
-    if (warp || d >= D) return;
+    };
+    const auto rebase = [&](float top) {                       // what the sums are relative to, 0 for -inf
+        const float base = top == -INFINITY ? 0.f : top, f = exp2f(M - base);
+        L *= f; A.x *= f; A.y *= f; A.z *= f; A.w *= f;
+        M = top;
+        return base;
+    };
+    for (int p0 = sub * kParts; p0 < n; p0 += W * kParts) {
+        float2 v[kParts];
+        float4 x[kParts];
 #pragma unroll
-    for (int w = 1; w < kJoinWarps; ++w) {
-        const float4 x = sums[w][lane];
-        A.x += x.x; A.y += x.y; A.z += x.z; A.w += x.w;
-        L += sl[w];
-    }
-    const float y[4] = {A.x, A.y, A.z, A.w};
+        for (int i = 0; i < kParts; ++i) {
+            const bool on = p0 + i < n;
+            v[i] = on ? ml[p0 + i] : make_float2(-INFINITY, 0.f);
+            x[i] = on && d < D ? *reinterpret_cast<const float4*>(acc + (long long)(p0 + i) * D + d) : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+        float top = M;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        const float z = L == 0.f ? 0.f : y[e] / L;
-        if (a.q_f32) static_cast<float*>(a.out)[(long long)row * D + d + e] = z;
-        else static_cast<__nv_bfloat16*>(a.out)[(long long)row * D + d + e] = __float2bfloat16(z);
+        for (int i = 0; i < kParts; ++i) top = fmaxf(top, v[i].x);
+        const float base = rebase(top);
+#pragma unroll
+        for (int i = 0; i < kParts; ++i) add(v[i], x[i], base);
     }
+    if constexpr (W > 1) {
+        sums[warp][lane] = A;
+        if (lane == 0) tops[warp] = make_float2(M, L);
+        __syncthreads();
+        if (sub) return;
+        float top = M;
+#pragma unroll
+        for (int w = 1; w < W; ++w) top = fmaxf(top, tops[warp + w].x);
+        const float base = rebase(top);
+#pragma unroll
+        for (int w = 1; w < W; ++w) add(tops[warp + w], sums[warp + w][lane], base);
+    }
+    if (row >= rows || d >= D) return;
+    const float z[4] = {L == 0.f ? 0.f : A.x / L, L == 0.f ? 0.f : A.y / L, L == 0.f ? 0.f : A.z / L, L == 0.f ? 0.f : A.w / L};
+    if (a.q_f32) *reinterpret_cast<float4*>(static_cast<float*>(a.out) + (long long)row * D + d) = make_float4(z[0], z[1], z[2], z[3]);
+    else *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(a.out) + (long long)row * D + d) = make_uint2(pack_bf16x2(z[0], z[1]), pack_bf16x2(z[2], z[3]));
+}
+cudaError_t launch_join(const StepArgs& a, cudaStream_t s) {
+    const long long rows = (long long)a.c.S * a.c.H * a.G;
+    const auto grid = [&](int W) { return dim3((unsigned)((rows * W + kJoinWarps - 1) / kJoinWarps)); };
+    if (a.parts <= 4) return launch_after(join_kernel<1>, grid(1), kJoinWarps * 32, 0, s, a);
+    if (a.parts <= 8) return launch_after(join_kernel<2>, grid(2), kJoinWarps * 32, 0, s, a);
+    return launch_after(join_kernel<8>, grid(8), kJoinWarps * 32, 0, s, a);
 }
 
 cudaError_t launch_step(const StepArgs& a, cudaStream_t s) {
@@ -409,7 +435,7 @@ int dsqg_paged_step(const dsqg_pages* cache, const void* q, const void* k_new, c
     }
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     cudaError_t e = paged_mma_supported(a) ? launch_paged_mma(a, s) : launch_step(a, s);
-    if (e == cudaSuccess && a.ml) e = launch_after(join_kernel, a.c.S * q_heads, kJoinWarps * 32, 0, s, a);
+    if (e == cudaSuccess && a.ml) e = launch_join(a, s);
     return status(e);
 }
 

@@ -3,7 +3,7 @@
 // A block takes a part of one sequence for up to 8 HT query heads of one key-value head, a warp every fourth tile of 16 positions of it.  Positions are
 // the 16 rows of mma.sync (m16n8k16, fp32 accumulators) and the query heads its 8 columns: S^T = K Q^T, softmax with a running maximum and sum per
 // column, O^T += V^T P^T.  A tile is one run of memory (a page keeps key and value of a position side by side): a warp copies its tiles to shared memory
-// with cp.async, some rounds ahead, 512 consecutive bytes an instruction, and waits for nobody but itself.  (Every lane copying the pieces that
+// with cp.async, two tiles ahead, 512 consecutive bytes an instruction, and waits for nobody but itself.  (Every lane copying the pieces that
 // it needs itself, 64 to 128 bytes a row: 68 us of copies alone for 4 sequences of 100001 positions, 4 x 8 heads of 128 in 8 bits, against 51.)  The
 // 16-byte pieces of a row are exchanged by s(row), so that the reads below are free of bank conflicts.  The contraction of a product, and the rows of
 // its result, may be permuted freely: key rows are the A operand as they lie (lane (g, t): rows g and g + 8, every fourth piece from t); of the value
@@ -49,8 +49,10 @@ template <int WORDS> __device__ __forceinline__ void load_shared(uint32_t from, 
 }
 // 2^x (2 ulp; results below 2^-126 become 0)
 __device__ __forceinline__ float exp2_fast(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
-__device__ __forceinline__ uint32_t half2_bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
-__device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) { return half2_bits(__floats2half2_rn(lo, hi)); }
+__device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
 
 // 8 x 8 elements of 16 bits, a pair of a row a lane: transposed.
 __device__ __forceinline__ uint32_t transposed(uint32_t x) {
@@ -61,7 +63,7 @@ __device__ __forceinline__ uint32_t transposed(uint32_t x) {
 // 2^(byte - top) for a scale byte that is at most top
 __device__ __forceinline__ float relative_scale(uint32_t byte, uint32_t top) { return __uint_as_float((uint32_t)max(127 + (int)byte - (int)top, 0) << 23); }
 
-template <int D, bool F8, int HT, int U, int STAGES>
+template <int D, bool F8, int HT, int STAGES>
 struct Cfg {
     static constexpr int SZ = F8 ? 1 : 2, ROW = 2 * D * SZ;              // bytes of an element, of a position
     static constexpr int KB = F8 ? (D % 64 == 0 ? 16 : 8) : 16;          // bytes of a piece of a key row: four lanes take 4 KB bytes
@@ -72,7 +74,7 @@ struct Cfg {
     static constexpr int STAGE = SOFF + (F8 ? 2 * kTile : 0);
     static constexpr bool EXCHANGE = ROW % 128 == 0;                     // rows of whole 128-byte lines
     static constexpr int HEADS = 8 * HT;
-    static constexpr int FIFO = kWarps * STAGES * U * STAGE, MERGE = kWarps * HEADS * (D + 2) * 4;
+    static constexpr int FIFO = kWarps * STAGES * STAGE, MERGE = kWarps * HEADS * (D + 2) * 4;
     static constexpr int BUF = FIFO > MERGE ? FIFO : MERGE;
     static constexpr int SMEM = BUF + 2 * D * SZ + 16;
     static constexpr int MT = D / 16;                                    // m-tiles of the output, and steps of the contraction over D
@@ -84,40 +86,44 @@ struct Cfg {
     }
 };
 
-// U tiles a round, STAGES - 1 rounds of copies ahead.
-template <int D, bool F8, int HT, int U, int STAGES, int CTAS>
+// STAGES - 1 tiles of copies ahead.
+template <int D, bool F8, int HT, int STAGES, int CTAS>
 __global__ void __launch_bounds__(kWarps * 32, CTAS) step_mma_kernel(const StepArgs a) {
-    using C = Cfg<D, F8, HT, U, STAGES>;
+    using C = Cfg<D, F8, HT, STAGES>;
     extern __shared__ __align__(16) char smem[];
     char* const fresh = smem + C::BUF;
     uint8_t* const fresh_scale = reinterpret_cast<uint8_t*>(fresh + 2 * D * C::SZ);
     stream_wait();
     const PageArgs& c = a.c;
     const int blocks_h = (a.G + C::HEADS - 1) / C::HEADS, hb = blockIdx.y % blocks_h, h = blockIdx.y / blocks_h, s = blockIdx.z, part = blockIdx.x;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+
+    // (column, row) of the table walk ahead of the tile that is asked for, so that the page's index is there when it is needed: the first while the length is
+    // on its way.
+    constexpr int STEP = kWarps * kTile;                       // positions from a warp's tile to its next
+    const int first_tile = part * a.chunk + warp * kTile;
+    const int32_t* const table = c.table + (long long)s * c.columns;
+    const int step_columns = STEP / c.page, step_rows = STEP % c.page;
+    int column = first_tile / c.page, row = first_tile % c.page, next_id = 0, next_row = 0;
+    const auto look = [&] {                                    // the page of the next tile
+        if (column < c.columns) next_id = __ldg(table + column);
+        next_row = row;
+        column += step_columns; row += step_rows;
+        if (row >= c.page) { row -= c.page; ++column; }
+    };
+    look();
     const Range r = range_of(a, s, part);
     if (part && r.first >= r.length) return;                   // part 0 always answers
     const int heads = min(C::HEADS, a.G - hb * C::HEADS);
     const long long q0 = ((long long)s * c.H + h) * a.G + hb * C::HEADS;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const bool has_new = a.k_new != nullptr && r.end == r.length && r.length > 0;
     const int last = has_new ? r.length - 1 : -1, old_end = has_new ? r.length - 1 : r.end;     // rows in front of old_end come from the pages
 
-    const uint32_t fifo = static_cast<uint32_t>(__cvta_generic_to_shared(smem)) + warp * STAGES * U * C::STAGE;
-    constexpr int STEP = kWarps * kTile;                       // positions from a warp's tile to its next
-    const int first_tile = r.first + warp * kTile, tiles = r.end > first_tile ? (r.end - first_tile + STEP - 1) / STEP : 0;
+    const uint32_t fifo = static_cast<uint32_t>(__cvta_generic_to_shared(smem)) + warp * STAGES * C::STAGE;
+    const int tiles = r.end > first_tile ? (r.end - first_tile + STEP - 1) / STEP : 0;
     bool bad = r.bad;
 
-    // ---- copies.  (column, row) of the table walk ahead of the tile that is asked for, so that the page's index is there when it is needed.
-    const int32_t* const table = c.table + (long long)s * c.columns;
-    const int step_columns = STEP / c.page, step_rows = STEP % c.page;
-    int walk = 0, column = first_tile / c.page, row = first_tile % c.page;
-    int next_id = 0, next_row = 0;
-    const auto look = [&] {                                    // the page of tile `walk`
-        if (walk < tiles) next_id = __ldg(table + column);
-        next_row = row;
-        ++walk; column += step_columns; row += step_rows;
-        if (row >= c.page) { row -= c.page; ++column; }
-    };
+    // ---- copies
     const auto issue = [&](int i, uint32_t st) {
         const int id = next_id, row_in = next_row;
         look();
@@ -136,14 +142,12 @@ __global__ void __launch_bounds__(kWarps * 32, CTAS) step_mma_kernel(const StepA
                 if (lane < kTile / 2) copy_async<4>(st + C::SOFF + lane * 4, reinterpret_cast<const char*>(c.scale) + row0 * 2 + lane * 4, true);
         }
     };
-    const auto issue_round = [&](int first, int slot) {
-#pragma unroll
-        for (int u = 0; u < U; ++u) issue(first + u, fifo + (slot * U + u) * C::STAGE);
+    const auto issue_tile = [&](int first, int slot) {
+        issue(first, fifo + slot * C::STAGE);
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
-    look();
 #pragma unroll
-    for (int i = 0; i < STAGES - 1; ++i) issue_round(i * U, i);
+    for (int i = 0; i < STAGES - 1; ++i) issue_tile(i, i);
 
     // ---- queries as the B operand: column g of tile n
     uint32_t qb[HT][C::MT][2];
@@ -205,80 +209,70 @@ __global__ void __launch_bounds__(kWarps * 32, CTAS) step_mma_kernel(const StepA
     int slot = 0;
 
 #pragma unroll 1
-    for (int i = 0; i < tiles; i += U) {
-        __syncwarp();                                          // every lane has read the round that the next copies replace
-        issue_round(i + (STAGES - 1) * U, slot == 0 ? STAGES - 1 : slot - 1);
+    for (int i = 0; i < tiles; ++i) {
+        __syncwarp();                                          // every lane has read the tile that the next copies replace
+        issue_tile(i + STAGES - 1, slot == 0 ? STAGES - 1 : slot - 1);
         asm volatile("cp.async.wait_group %0;" :: "n"(STAGES - 1) : "memory");
         __syncwarp();
-        const uint32_t st0 = fifo + slot * U * C::STAGE;
+        const uint32_t st0 = fifo + slot * C::STAGE;
         slot = slot == STAGES - 1 ? 0 : slot + 1;
-        const int p0 = first_tile + i * STEP;                  // tile u of the round: positions p0 + u STEP on
-        if (last >= p0 && last < p0 + (U - 1) * STEP + kTile && (last - p0) % STEP < kTile) {      // the new token's row: from where new_row left it
-            const int key = (last - p0) % STEP;
-            char* const to = smem + (st0 - static_cast<uint32_t>(__cvta_generic_to_shared(smem))) + (last - p0) / STEP * C::STAGE;
+        const int p0 = first_tile + i * STEP;                  // the tile has positions p0 on
+        if (last >= p0 && last < p0 + kTile) {                 // the new token's row: from where new_row left it
+            const int key = last - p0;
+            char* const to = smem + (st0 - static_cast<uint32_t>(__cvta_generic_to_shared(smem)));
             if (lane * 16 < C::ROW) *reinterpret_cast<uint4*>(to + C::at(key, lane * 16)) = *reinterpret_cast<const uint4*>(fresh + lane * 16);
             if (F8 && lane < 2) to[C::SOFF + 2 * key + lane] = fresh_scale[lane];
             __syncwarp();
         }
         // ---- scores: positions g and g + 8 of a tile, heads 2 t and 2 t + 1; two chains of products each, for they wait for one another
-        float sc[U][HT][4];
+        float sc[HT][4];
+        float odd[HT][4];
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const uint32_t st = st0 + u * C::STAGE;
-            float odd[HT][4];
+        for (int n = 0; n < HT; ++n)
 #pragma unroll
-            for (int n = 0; n < HT; ++n)
+            for (int e = 0; e < 4; ++e) sc[n][e] = odd[n][e] = 0.f;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) sc[u][n][e] = odd[n][e] = 0.f;
+        for (int k = 0; k < C::KP; ++k) {
+            uint32_t w[2][C::KB / 4];
+            load_shared(st0 + C::at(g, (4 * k + t) * C::KB), w[0]);
+            load_shared(st0 + C::at(g, (4 * k + t) * C::KB) + 8 * C::ROW, w[1]);      // s(g + 8) = s(g)
+            constexpr int N = F8 ? C::KB / 4 : 2;          // steps of a piece
 #pragma unroll
-            for (int k = 0; k < C::KP; ++k) {
-                uint32_t w[2][C::KB / 4];
-                load_shared(st + C::at(g, (4 * k + t) * C::KB), w[0]);
-                load_shared(st + C::at(g, (4 * k + t) * C::KB) + 8 * C::ROW, w[1]);      // s(g + 8) = s(g)
-                constexpr int N = F8 ? C::KB / 4 : 2;          // steps of a piece
+            for (int e = 0; e < N; ++e) {
+                uint32_t ka[4];
+                if constexpr (F8) { e4m3x4_half2(w[0][e], ka[0], ka[2]); e4m3x4_half2(w[1][e], ka[1], ka[3]); }
+                else { ka[0] = w[0][2 * e]; ka[1] = w[1][2 * e]; ka[2] = w[0][2 * e + 1]; ka[3] = w[1][2 * e + 1]; }
 #pragma unroll
-                for (int e = 0; e < N; ++e) {
-                    uint32_t ka[4];
-                    if constexpr (F8) { e4m3x4_half2(w[0][e], ka[0], ka[2]); e4m3x4_half2(w[1][e], ka[1], ka[3]); }
-                    else { ka[0] = w[0][2 * e]; ka[1] = w[1][2 * e]; ka[2] = w[0][2 * e + 1]; ka[3] = w[1][2 * e + 1]; }
-#pragma unroll
-                    for (int n = 0; n < HT; ++n) mma<F8>(e & 1 ? odd[n] : sc[u][n], ka, qb[n][k * N + e][0], qb[n][k * N + e][1]);
-                }
+                for (int n = 0; n < HT; ++n) mma<F8>(e & 1 ? odd[n] : sc[n], ka, qb[n][k * N + e][0], qb[n][k * N + e][1]);
             }
-#pragma unroll
-            for (int n = 0; n < HT; ++n)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) sc[u][n][e] += odd[n][e];
         }
+#pragma unroll
+        for (int n = 0; n < HT; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sc[n][e] += odd[n][e];
         // ---- softmax.  A score is the product times its row's scale (ks), in units of 1 / fs; m is in the same units.
-        bool valid[U][2];
-        float ks[U][2], vs[U][2];
+        bool valid[2];
+        float ks[2], vs[2];
 #pragma unroll
-        for (int u = 0; u < U; ++u)
-#pragma unroll
-            for (int j = 0; j < 2; ++j) { valid[u][j] = p0 + u * STEP + 8 * j + g < r.end; ks[u][j] = vs[u][j] = 1.f; }
+        for (int j = 0; j < 2; ++j) { valid[j] = p0 + 8 * j + g < r.end; ks[j] = vs[j] = 1.f; }
         if constexpr (F8) {
-            uint32_t kb[U][2], vb[U][2], top = 0u;
+            uint32_t kb[2], vb[2], top = 0u;
             bool nan = false;
 #pragma unroll
-            for (int u = 0; u < U; ++u)
-#pragma unroll
-                for (int j = 0; j < 2; ++j) {
+            for (int j = 0; j < 2; ++j) {
                     uint16_t b;
-                    asm volatile("ld.shared.u16 %0, [%1];" : "=h"(b) : "r"(st0 + u * C::STAGE + C::SOFF + 2 * (8 * j + g)) : "memory");
-                    if (!valid[u][j]) b = 0;
-                    kb[u][j] = b & 255u; vb[u][j] = b >> 8;
-                    nan |= kb[u][j] == 255u || vb[u][j] == 255u;
-                    top = max(top, vb[u][j]);
-                    ks[u][j] = __uint_as_float(kb[u][j] << 23);               // a byte of 0 (2^-127, which no row of this library has): 0
+                    asm volatile("ld.shared.u16 %0, [%1];" : "=h"(b) : "r"(st0 + C::SOFF + 2 * (8 * j + g)) : "memory");
+                    if (!valid[j]) b = 0;
+                    kb[j] = b & 255u; vb[j] = b >> 8;
+                    nan |= kb[j] == 255u || vb[j] == 255u;
+                    top = max(top, vb[j]);
+                    ks[j] = __uint_as_float(kb[j] << 23);               // a byte of 0 (2^-127, which no row of this library has): 0
                 }
             const bool some_nan = __any_sync(0xffffffffu, nan);
             if (some_nan) {
                 top = 0u;
 #pragma unroll
-                for (int u = 0; u < U; ++u)
-#pragma unroll
-                    for (int j = 0; j < 2; ++j) top = max(top, vb[u][j] == 255u ? 0u : vb[u][j]);
+                for (int j = 0; j < 2; ++j) top = max(top, vb[j] == 255u ? 0u : vb[j]);
             }
             top = __reduce_max_sync(0xffffffffu, top);
             if (top > vtop) {                                  // rarely: the scales of a head's values are much alike
@@ -292,29 +286,25 @@ __global__ void __launch_bounds__(kWarps * 32, CTAS) step_mma_kernel(const StepA
                 vtop = top;
             }
 #pragma unroll
-            for (int u = 0; u < U; ++u)
-#pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    vs[u][j] = relative_scale(vb[u][j], vtop);
+            for (int j = 0; j < 2; ++j) {
+                    vs[j] = relative_scale(vb[j], vtop);
                     if (some_nan) {
-                        if (kb[u][j] == 255u) ks[u][j] = __uint_as_float(0x7fc00000u);
-                        if (vb[u][j] == 255u) vs[u][j] = __uint_as_float(0x7fc00000u);
+                        if (kb[j] == 255u) ks[j] = __uint_as_float(0x7fc00000u);
+                        if (vb[j] == 255u) vs[j] = __uint_as_float(0x7fc00000u);
                     }
                 }
         }
-        uint32_t pb[U][HT][2];
+        uint32_t pb[HT][2];
 #pragma unroll
         for (int n = 0; n < HT; ++n) {
             float mx[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-            for (int u = 0; u < U; ++u)
-#pragma unroll
-                for (int x = 0; x < 2; ++x)
+            for (int x = 0; x < 2; ++x)
 #pragma unroll
                     for (int j = 0; j < 2; ++j) {
-                        float& v = sc[u][n][2 * j + x];
-                        if constexpr (F8) v *= ks[u][j];
-                        v = valid[u][j] ? v : -INFINITY;
+                        float& v = sc[n][2 * j + x];
+                        if constexpr (F8) v *= ks[j];
+                        v = valid[j] ? v : -INFINITY;
                         mx[x] = fmaxf(mx[x], v);
                     }
             if (__any_sync(0xffffffffu, mx[0] > lim[n][0] || mx[1] > lim[n][1])) {
@@ -332,29 +322,25 @@ __global__ void __launch_bounds__(kWarps * 32, CTAS) step_mma_kernel(const StepA
                 }
             }
 #pragma unroll
-            for (int u = 0; u < U; ++u)
-#pragma unroll
-                for (int j = 0; j < 2; ++j) {
+            for (int j = 0; j < 2; ++j) {
                     float x[2];
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
-                        x[e] = exp2_fast(fmaf(sc[u][n][2 * j + e], fs[n][e], -base[n][e]));
+                        x[e] = exp2_fast(fmaf(sc[n][2 * j + e], fs[n][e], -base[n][e]));
                         l[n][e] += x[e];
-                        if constexpr (F8) x[e] *= vs[u][j];
+                        if constexpr (F8) x[e] *= vs[j];
                     }
                     // to 16 bits, as the operand of the product: relative 2^-9 (bf16) or 2^-12 (f16) on terms that add up, within the result's own rounding
-                    pb[u][n][j] = transposed(F8 ? pack_f16x2(x[0], x[1]) : pack_bf16x2(x[0], x[1]));
+                    pb[n][j] = transposed(F8 ? pack_f16x2(x[0], x[1]) : pack_bf16x2(x[0], x[1]));
                 }
         }
         // ---- O^T += V^T P^T: rows g and g + 8 of m-tile (k VE + e) / 2 are d = 8 VE k + VE g + e and the next
 #pragma unroll
-        for (int u = 0; u < U; ++u)
-#pragma unroll
-            for (int k = 0; k < C::VP; ++k) {
+        for (int k = 0; k < C::VP; ++k) {
                 uint32_t w[4][C::VB / 4];
 #pragma unroll
                 for (int j = 0; j < 4; ++j)                    // positions 2 t, 2 t + 1 (+ 8)
-                    load_shared(st0 + u * C::STAGE + C::at(2 * t + (j & 1), D * C::SZ + (8 * k + g) * C::VB) + 8 * (j >> 1) * C::ROW, w[j]);
+                    load_shared(st0 + C::at(2 * t + (j & 1), D * C::SZ + (8 * k + g) * C::VB) + 8 * (j >> 1) * C::ROW, w[j]);
 #pragma unroll
                 for (int x = 0; x < C::VB / 4; ++x) {
                     if constexpr (F8) {
@@ -364,13 +350,13 @@ __global__ void __launch_bounds__(kWarps * 32, CTAS) step_mma_kernel(const StepA
                             e4m3x4_half2(__byte_perm(w[0][x], w[1][x], y ? 0x7362 : 0x5140), va[0], va[1]);
                             e4m3x4_half2(__byte_perm(w[2][x], w[3][x], y ? 0x7362 : 0x5140), va[2], va[3]);
 #pragma unroll
-                            for (int n = 0; n < HT; ++n) mma<true>(o[n][(k * C::VE + 4 * x) / 2 + y], va, pb[u][n][0], pb[u][n][1]);
+                            for (int n = 0; n < HT; ++n) mma<true>(o[n][(k * C::VE + 4 * x) / 2 + y], va, pb[n][0], pb[n][1]);
                         }
                     } else {
                         const uint32_t va[4] = {__byte_perm(w[0][x], w[1][x], 0x5410), __byte_perm(w[0][x], w[1][x], 0x7632),
                                                 __byte_perm(w[2][x], w[3][x], 0x5410), __byte_perm(w[2][x], w[3][x], 0x7632)};
 #pragma unroll
-                        for (int n = 0; n < HT; ++n) mma<false>(o[n][(k * C::VE + 2 * x) / 2], va, pb[u][n][0], pb[u][n][1]);
+                        for (int n = 0; n < HT; ++n) mma<false>(o[n][(k * C::VE + 2 * x) / 2], va, pb[n][0], pb[n][1]);
                     }
                 }
             }
@@ -416,9 +402,9 @@ __global__ void __launch_bounds__(kWarps * 32, CTAS) step_mma_kernel(const StepA
     }
 }
 
-template <int D, bool F8, int HT, int U, int STAGES, int CTAS> cudaError_t launch_one(const StepArgs& a, cudaStream_t s) {
-    using C = Cfg<D, F8, HT, U, STAGES>;
-    auto kern = step_mma_kernel<D, F8, HT, U, STAGES, CTAS>;
+template <int D, bool F8, int HT, int STAGES, int CTAS> cudaError_t launch_one(const StepArgs& a, cudaStream_t s) {
+    using C = Cfg<D, F8, HT, STAGES>;
+    auto kern = step_mma_kernel<D, F8, HT, STAGES, CTAS>;
     static bool ready[64] = {};                                // per device: the attribute is set once
     int dev = 0;
     if (cudaError_t e = cudaGetDevice(&dev)) return e;
@@ -430,9 +416,10 @@ template <int D, bool F8, int HT, int U, int STAGES, int CTAS> cudaError_t launc
 }
 template <int D, bool F8> cudaError_t launch_width(const StepArgs& a, cudaStream_t s) {
     // Two CTAs of four warps and 8-KB tiles in bf16, four in 8 bits, two tiles ahead each (us, 64 sequences up to 4096, 8 x 4 heads of 128 in bf16 / 4 up to
-    // 100001, 4 x 8 heads of 128 in 8 bits: 90.9 / 59.6; one tile ahead and three CTAs 91.5 / 67.8; two tiles a round, three CTAs, 8 bits 67.8).
-    if (a.G > 8) return launch_one<D, F8, 2, 1, 3, 2>(a, s);
-    return launch_one<D, F8, 1, 1, 3, F8 ? 4 : 2>(a, s);
+    // 100001, 4 x 8 heads of 128 in 8 bits: 90.9 / 59.6; one tile ahead and three CTAs 91.5 / 67.8; two tiles a round, three CTAs, 8 bits 67.8;
+    // tiles by the copy engine through a swizzled tensor map 92.8 / 58.4).
+    if (a.G > 8) return launch_one<D, F8, 2, 3, 2>(a, s);
+    return launch_one<D, F8, 1, 3, F8 ? 4 : 2>(a, s);
 }
 template <bool F8> cudaError_t launch_type(const StepArgs& a, cudaStream_t s) {
     switch (a.c.D) {
