@@ -1,4 +1,5 @@
 // The paged cache written from and read back to token-major tensors, and one new token's attention to it on CUDA cores, for every type and width.
+#include <algorithm>
 #include <cmath>
 
 #include "dsqg_paged.cuh"
@@ -342,13 +343,15 @@ cudaError_t launch_step(const StepArgs& a, cudaStream_t s) {
 inline bool bad(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) != 0; }
 inline int status(cudaError_t e) { return e == cudaSuccess ? DSQG_OK : DSQG_ERR_CUDA; }
 
-// The positions of a part: a multiple of 64, from the sizes alone.
+// The positions of a part: a multiple of 64, from the sizes alone.  Of blocks that run at once (`an_sm` per SM) about 85 % shall have work if lengths are spread
+// evenly up to the longest: below all of them, for one block too many takes as long as twice as many.  From 16 sequences on, which differ more, twice as many
+// parts.  Up to 2048 positions a part.  (us, with one part of the longest for every block that runs at once, whatever the lengths / with this: 16 sequences
+// up to 8192, 8 x 4 heads of 128 in 8 bits, 44 / 34; 4 up to 20000, 4 x 8 heads in 8 bits, 21.7 / 19.1; one of 4096, 8 x 4 heads in bf16, 10.5 / 7.6.)
 struct Split { int chunk, parts; };
-inline Split split_for(int S, int H, int G, int limit) {
-    const long long pairs = (long long)S * H * ((G + 15) / 16);
-    const long long most = (limit + 63) / 64;                                  // in units of 64 positions
-    long long units = (pairs * most + 148 * 4 - 1) / (148 * 4);                // as many blocks as run at once ...
-    if (units > 32) units = 32;                                                // ... of up to 2048 positions: sequences differ in length
+inline Split split_for(int S, int H, int G, int limit, int an_sm) {
+    const double pairs = (double)S * H * ((G + 15) / 16), share = (S + 1) / (2.0 * S), blocks = 148 * an_sm * 0.85 * (S < 16 ? 1 : 2);
+    const long long most = ((long long)limit + 63) / 64;                       // in units of 64 positions
+    long long units = (long long)std::ceil(std::min(pairs * most * share / blocks, 32.0));
     const long long least = (most + 1023) / 1024;                              // no more than 1024 parts
     if (units < least) units = least;
     if (units < 1) units = 1;
@@ -358,6 +361,8 @@ inline Split split_for(int S, int H, int G, int limit) {
     if (r.parts < 1) r.parts = 1;
     return r;
 }
+// Blocks of the kernel that a step takes that an SM holds.
+inline int blocks_an_sm(bool mma, int G, bool f8) { return mma && (G > 8 || !f8) ? 2 : 4; }
 
 // A description of a cache that kernels may use.
 int page_args(const dsqg_pages* c, PageArgs* a) {
@@ -408,8 +413,8 @@ int dsqg_paged_read(const dsqg_pages* cache, void* k, void* v, const int32_t* cu
 
 size_t dsqg_paged_step_scratch_bytes(int sequences, int heads, int q_heads, int D, int max_length) {
     if (sequences < 1 || heads < 1 || q_heads < heads || q_heads % heads || D < 1 || max_length < 0) return 0;
-    const Split p = split_for(sequences, heads, q_heads / heads, max_length);
-    return p.parts == 1 ? 0 : (size_t)sequences * q_heads * p.parts * (D + 2) * 4;
+    const int parts = std::max(split_for(sequences, heads, q_heads / heads, max_length, 2).parts, split_for(sequences, heads, q_heads / heads, max_length, 4).parts);
+    return parts == 1 ? 0 : (size_t)sequences * q_heads * parts * (D + 2) * 4;
 }
 
 int dsqg_paged_step(const dsqg_pages* cache, const void* q, const void* k_new, const void* v_new, const int32_t* lengths, int q_heads, int max_length, float scale,
@@ -425,7 +430,8 @@ int dsqg_paged_step(const dsqg_pages* cache, const void* q, const void* k_new, c
     a.limit = max_length;
     a.q = q; a.k_new = k_new; a.v_new = v_new; a.lengths = lengths; a.out = out; a.G = q_heads / a.c.H; a.q_f32 = dtype == DSQG_DTYPE_F32;
     a.scale = (scale > 0.f ? scale : 1.0f / sqrtf((float)a.c.D)) * 1.4426950408889634f;
-    const Split p = split_for(a.c.S, a.c.H, a.G, a.limit);
+    const bool mma = paged_mma_supported(a);
+    const Split p = split_for(a.c.S, a.c.H, a.G, a.limit, blocks_an_sm(mma, a.G, a.c.dtype == DSQG_DTYPE_E4M3));
     a.chunk = p.chunk; a.parts = p.parts; a.ml = nullptr; a.acc = nullptr;
     if (p.parts > 1) {
         const size_t rows = (size_t)a.c.S * q_heads * p.parts;
@@ -434,7 +440,7 @@ int dsqg_paged_step(const dsqg_pages* cache, const void* q, const void* k_new, c
         a.acc = static_cast<float*>(scratch); a.ml = reinterpret_cast<float2*>(a.acc + rows * a.c.D);
     }
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
-    cudaError_t e = paged_mma_supported(a) ? launch_paged_mma(a, s) : launch_step(a, s);
+    cudaError_t e = mma ? launch_paged_mma(a, s) : launch_step(a, s);
     if (e == cudaSuccess && a.ml) e = launch_join(a, s);
     return status(e);
 }

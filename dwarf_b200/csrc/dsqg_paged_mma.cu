@@ -415,9 +415,9 @@ template <int D, bool F8, int HT, int STAGES, int CTAS> cudaError_t launch_one(c
     return launch_after(kern, dim3(a.parts, a.c.H * ((a.G + C::HEADS - 1) / C::HEADS), a.c.S), kWarps * 32, C::SMEM, s, a);
 }
 template <int D, bool F8> cudaError_t launch_width(const StepArgs& a, cudaStream_t s) {
-    // Two CTAs of four warps and 8-KB tiles in bf16, four in 8 bits, two tiles ahead each (us, 64 sequences up to 4096, 8 x 4 heads of 128 in bf16 / 4 up to
-    // 100001, 4 x 8 heads of 128 in 8 bits: 90.9 / 59.6; one tile ahead and three CTAs 91.5 / 67.8; two tiles a round, three CTAs, 8 bits 67.8;
-    // tiles by the copy engine through a swizzled tensor map 92.8 / 58.4).
+    // Two CTAs of four warps and 8-KB tiles in bf16, four in 8 bits, two tiles ahead each: 87 us for 64 sequences up to 4096, 8 x 4 heads of 128 in bf16 (84 at
+    // the rate of a copy), 58 us for 4 up to 100001, 4 x 8 heads of 128 in 8 bits (44).  Three CTAs and one tile ahead cost 1 % and 14 % more, two tiles a round
+    // with three CTAs 14 % in 8 bits; tiles by the copy engine through a swizzled tensor map 2 % more in bf16 and 2 % less in 8 bits.
     if (a.G > 8) return launch_one<D, F8, 2, 3, 2>(a, s);
     return launch_one<D, F8, 1, 3, F8 ? 4 : 2>(a, s);
 }
