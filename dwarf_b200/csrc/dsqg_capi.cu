@@ -26,6 +26,18 @@ static int cuda_fail(cudaError_t e) {
     return DSQG_ERR_CUDA;
 }
 
+int cuda_status(cudaError_t e) { return e == cudaSuccess ? DSQG_OK : cuda_fail(e); }
+cudaError_t allow_shared(const void* kernel, int bytes, std::atomic<unsigned long long>& done) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    const unsigned long long bit = dev < 64 ? 1ull << dev : 0ull;
+    if (e != cudaSuccess || (done.load(std::memory_order_relaxed) & bit)) return e;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_relaxed);
+    else cudaGetLastError();
+    return e;
+}
+
 static inline bool misaligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) != 0; }
 
 // Validates the offsets and splits them into the dense run and the sparse taps.

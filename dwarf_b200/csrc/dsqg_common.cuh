@@ -1,6 +1,7 @@
 // Shared declarations for the DSQG CUDA sources (sm_100a).
 #pragma once
 
+#include <atomic>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
@@ -119,6 +120,11 @@ inline cudaError_t launch_clusters_after(unsigned cluster, void (*kern)(Params..
 __device__ __forceinline__ void wait_ahead() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void let_next_in() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void stream_wait() { wait_ahead(); let_next_in(); }
+
+// What a C entry returns; the error's text is kept for dsqg_last_cuda_error.
+int cuda_status(cudaError_t e);
+// Lets a kernel have more than 48 KB of shared memory a block: once per device (a bit of `done`).
+cudaError_t allow_shared(const void* kernel, int bytes, std::atomic<unsigned long long>& done);
 
 // Launchers (defined in the .cu files; return a cudaError_t from the launch).
 cudaError_t launch_fwd(const FwdArgs& a, const Taps& t, int dtype, cudaStream_t s);   // dispatcher

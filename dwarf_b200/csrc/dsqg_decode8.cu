@@ -6,7 +6,8 @@
 // of 64 columns are six rounds.  The step attends to what the ring holds: the new token's rows are quantised first, and tap 0 reads them.
 //
 // 256 sequences, 12 heads of 64, 43 taps: HBM's floor is 2.9 us, the dependent chain of one wave of warps (write head, rows, softmax, result) the rest.
-// With the rows of a step in registers (157 of them, 12 warps an SM, two waves) it took 10.6.
+// With the rows of a step in registers (157 of them, 12 warps an SM, two waves) this form took 10.6.  bf16 queries without scale_embed take the form on tensor
+// cores further down: 7.9.
 #include "dsqg_rows8.cuh"
 
 namespace dsqg {
@@ -211,7 +212,7 @@ decode8_kernel(const DecodeArgs a, uint8_t* __restrict__ scale, const Taps t) {
 // Taps are the 16 rows of mma.sync (m16n8k16, f16 in, fp32 sums), the query stands in all eight columns: scores = K q without a shuffle, and after the softmax
 // O^T += V^T p without one, p turned from a result into an operand by movmatrix.  e4m3 becomes f16 exactly; the query becomes f16 after a power of two
 // that brings its largest element to [1, 2); the keys' scales multiply the scores, the values' scales the probabilities, relative to the largest scale
-// of the step.  What bounds the step is instructions, not memory: some 700 a warp instead of the 1730 of the form above, whose rows go to fp32 one by one.
+// of the step.  What bounds the step is instructions, not memory: some 1180 a warp instead of the 1730 of the form above, whose rows go to fp32 one by one.
 // A lane asks for the pieces of key rows g and g + 8 that it needs itself (lane (g, t): piece t); value rows go to shared memory as rows, even ones in
 // front of odd ones and pieces exchanged so that rows 2 t, 2 t + 1, 2 t + 8, 2 t + 9 are read without bank conflicts.
 template <int D> struct Mma {
@@ -236,7 +237,7 @@ template <int WORDS> __device__ __forceinline__ void words_of(const void* p, uin
 }
 
 template <int D, bool PDL>
-__global__ void __launch_bounds__(Mma<D>::W * 32, D == 128 ? 6 : 6) decode8_mma_kernel(const DecodeArgs a, uint8_t* __restrict__ scale, const Taps t) {
+__global__ void __launch_bounds__(Mma<D>::W * 32, 6) decode8_mma_kernel(const DecodeArgs a, uint8_t* __restrict__ scale, const Taps t) {
     using C = Mma<D>;
     constexpr int TILES = C::TILES, KP = C::KP, KB = C::KB, VEC = D / 4, STEPS = D / 16, E = KB / 4;
     if constexpr (!PDL) stream_wait();
@@ -516,8 +517,7 @@ int dsqg_ring_prefill_e4m3(const void* k, const void* v, void* kv_ring, void* kv
     const long long threads = (long long)S * H * (N < R ? N : R) * 2 * lpr;        // at least S
     const unsigned blocks = (unsigned)((threads + 255) / 256);
     auto kern = lpr == 1 ? ring_prefill8_kernel<1> : lpr == 2 ? ring_prefill8_kernel<2> : lpr == 4 ? ring_prefill8_kernel<4> : lpr == 8 ? ring_prefill8_kernel<8> : ring_prefill8_kernel<16>;
-    return launch_after(kern, blocks, 256, 0, static_cast<cudaStream_t>(stream), k, v, static_cast<uint8_t*>(kv_ring), static_cast<uint8_t*>(kv_scale), head, fill, S, H, N, R, D, dtype)
-        == cudaSuccess ? DSQG_OK : DSQG_ERR_CUDA;
+    return cuda_status(launch_after(kern, blocks, 256, 0, static_cast<cudaStream_t>(stream), k, v, static_cast<uint8_t*>(kv_ring), static_cast<uint8_t*>(kv_scale), head, fill, S, H, N, R, D, dtype));
 }
 
 int dsqg_dequantize_rows(const void* x, const void* scale, void* out, long long rows, int D, int dtype, void* stream) {
@@ -525,8 +525,8 @@ int dsqg_dequantize_rows(const void* x, const void* scale, void* out, long long 
     if (dtype != DSQG_DTYPE_BF16 && dtype != DSQG_DTYPE_F32) return DSQG_ERR_BAD_DTYPE;
     if (rows < 1 || D < 8 || D % 8 || rows * (D / 8) > 0x7fffffffLL * 256) return DSQG_ERR_BAD_SHAPE;
     if (bad(x) || bad(out)) return DSQG_ERR_MISALIGNED;
-    return launch_after(dequantize_kernel, (unsigned)((rows * (D / 8) + 255) / 256), 256, 0, static_cast<cudaStream_t>(stream), static_cast<const uint8_t*>(x),
-                        static_cast<const uint8_t*>(scale), out, rows, D, dtype) == cudaSuccess ? DSQG_OK : DSQG_ERR_CUDA;
+    return cuda_status(launch_after(dequantize_kernel, (unsigned)((rows * (D / 8) + 255) / 256), 256, 0, static_cast<cudaStream_t>(stream), static_cast<const uint8_t*>(x),
+                        static_cast<const uint8_t*>(scale), out, rows, D, dtype));
 }
 
 }  // extern "C"

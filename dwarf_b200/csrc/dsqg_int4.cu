@@ -278,15 +278,9 @@ template <bool F8, int NT, int RT, int GC, int SUBS> cudaError_t launch_one(Int4
     constexpr int FIFO = kWarps * kStages * RT * 16 * 64 * SUBS, RED = kWarps * 8 * NT * (16 * RT + 1) * 4;
     constexpr int SMEM = FIFO > RED ? FIFO : RED;
     auto kern = int4_kernel<F8, NT, RT, GC, SUBS>;
-    if (SMEM > 48 * 1024) {
-        static bool ready[64] = {};                            // per device: the attribute is set once
-        int dev = 0;
-        if (cudaError_t e = cudaGetDevice(&dev)) return e;
-        if (dev < 0 || dev >= 64 || !ready[dev]) {
-            if (cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM)) { cudaGetLastError(); return e; }
-            if (dev >= 0 && dev < 64) ready[dev] = true;
-        }
-    }
+    static std::atomic<unsigned long long> done{0};
+    if (SMEM > 48 * 1024)
+        if (cudaError_t e = allow_shared(reinterpret_cast<const void*>(kern), SMEM, done)) return e;
     const int units = (a.N + 16 * RT - 1) / (16 * RT), cols = (a.K + 128 * SUBS - 1) / (128 * SUBS);
     a.ks = 1;
     while (a.ks < kWarps && a.ks < cols && units * a.ks < 148 * 12) a.ks *= 2;
@@ -326,7 +320,7 @@ int dsqg_int4_linear(const void* x, const void* x_scale, const void* weight, con
     const Int4Args a = {x, static_cast<const uint8_t*>(x_scale), static_cast<const uint8_t*>(weight), static_cast<const __nv_bfloat16*>(scales), bias,
                         static_cast<__nv_bfloat16*>(y), M, N, K, K / group};
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
-    return (dtype == DSQG_DTYPE_E4M3 ? launch_type<true>(a, group, s) : launch_type<false>(a, group, s)) == cudaSuccess ? DSQG_OK : DSQG_ERR_CUDA;
+    return cuda_status(dtype == DSQG_DTYPE_E4M3 ? launch_type<true>(a, group, s) : launch_type<false>(a, group, s));
 }
 
 }  // extern "C"

@@ -414,7 +414,6 @@ __global__ void __launch_bounds__(1024) dw_kernel(const float* __restrict__ part
 }
 
 inline bool bad(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) != 0; }
-inline int status(cudaError_t e) { return e == cudaSuccess ? DSQG_OK : DSQG_ERR_CUDA; }
 inline bool bad_rows(long long rows, int D) { return rows < 1 || D < 1 || rows > 0x7fffffffLL || rows * D > 0x7fffffffffLL; }
 inline bool bad_type(int t) { return t != DSQG_DTYPE_BF16 && t != DSQG_DTYPE_F32; }
 
@@ -471,13 +470,13 @@ int dsqg_rms_norm_fwd(const dsqg_rms_norm* p, void* stream) {
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     const long long per = rows_per_block(shape);
     const unsigned blocks = (unsigned)((p->rows + per - 1) / per);
-    if (!shape.v) return status(launch_after(rms_fwd_wide_kernel, blocks, 1024, 0, s, a));
+    if (!shape.v) return cuda_status(launch_after(rms_fwd_wide_kernel, blocks, 1024, 0, s, a));
     cudaError_t e = cudaSuccess;
     const bool s32 = p->residual && p->stream_dtype == DSQG_DTYPE_F32;
 #define DSQG_RUN(ODD, X32, S32, TPR, V) e = launch_after(rms_fwd_kernel<ODD, X32, S32, TPR, V>, blocks, TPR < kThreads ? kThreads : TPR, 0, s, a)
     if (p->D % 8) { DSQG_NORM_TYPES(shape, true, a.x_f32, s32, DSQG_RUN) } else { DSQG_NORM_TYPES(shape, false, a.x_f32, s32, DSQG_RUN) }
 #undef DSQG_RUN
-    return status(e);
+    return cuda_status(e);
 }
 
 size_t dsqg_rms_norm_bwd_scratch_bytes(long long rows, int D) {
@@ -510,7 +509,7 @@ int dsqg_rms_norm_bwd(const dsqg_rms_norm* p, const void* dy, const void* dh, vo
 #undef DSQG_RUN
     }
     if (e == cudaSuccess && dweight) e = launch_after(dw_kernel, (p->D + 31) / 32, 1024, 0, s, static_cast<const float*>(scratch), dweight, blocks, p->D);
-    return status(e);
+    return cuda_status(e);
 }
 
 }  // extern "C"

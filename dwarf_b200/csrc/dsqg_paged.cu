@@ -341,7 +341,6 @@ cudaError_t launch_step(const StepArgs& a, cudaStream_t s) {
 }
 
 inline bool bad(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) != 0; }
-inline int status(cudaError_t e) { return e == cudaSuccess ? DSQG_OK : DSQG_ERR_CUDA; }
 
 // The positions of a part: a multiple of 64, from the sizes alone.  Of blocks that run at once (`an_sm` per SM) about 85 % shall have work if lengths are spread
 // evenly up to the longest: below all of them, for one block too many takes as long as twice as many.  From 16 sequences on, which differ more, twice as many
@@ -401,14 +400,14 @@ int dsqg_paged_write(const dsqg_pages* cache, const void* k, const void* v, long
                      const int32_t* cu_seqlens, const int32_t* start, long long tokens, int dtype, void* stream) {
     MoveArgs a;
     if (int rc = move_args(cache, cu_seqlens, start, const_cast<void*>(k), const_cast<void*>(v), k_token, k_head, v_token, v_head, tokens, dtype, &a)) return rc;
-    return status(launch_move_heads<true>(a, static_cast<cudaStream_t>(stream)));
+    return cuda_status(launch_move_heads<true>(a, static_cast<cudaStream_t>(stream)));
 }
 
 int dsqg_paged_read(const dsqg_pages* cache, void* k, void* v, const int32_t* cu_seqlens, const int32_t* start, long long tokens, int dtype, void* stream) {
     MoveArgs a;
     const long long D = cache ? cache->D : 0, HD = cache ? D * cache->heads : 0;
     if (int rc = move_args(cache, cu_seqlens, start, k, v, HD, D, HD, D, tokens, dtype, &a)) return rc;
-    return status(launch_move_heads<false>(a, static_cast<cudaStream_t>(stream)));
+    return cuda_status(launch_move_heads<false>(a, static_cast<cudaStream_t>(stream)));
 }
 
 size_t dsqg_paged_step_scratch_bytes(int sequences, int heads, int q_heads, int D, int max_length) {
@@ -442,7 +441,7 @@ int dsqg_paged_step(const dsqg_pages* cache, const void* q, const void* k_new, c
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     cudaError_t e = mma ? launch_paged_mma(a, s) : launch_step(a, s);
     if (e == cudaSuccess && a.ml) e = launch_join(a, s);
-    return status(e);
+    return cuda_status(e);
 }
 
 }  // extern "C"

@@ -405,13 +405,8 @@ __global__ void __launch_bounds__(kWarps * 32, CTAS) step_mma_kernel(const StepA
 template <int D, bool F8, int HT, int STAGES, int CTAS> cudaError_t launch_one(const StepArgs& a, cudaStream_t s) {
     using C = Cfg<D, F8, HT, STAGES>;
     auto kern = step_mma_kernel<D, F8, HT, STAGES, CTAS>;
-    static bool ready[64] = {};                                // per device: the attribute is set once
-    int dev = 0;
-    if (cudaError_t e = cudaGetDevice(&dev)) return e;
-    if (dev < 0 || dev >= 64 || !ready[dev]) {
-        if (cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM)) { cudaGetLastError(); return e; }
-        if (dev >= 0 && dev < 64) ready[dev] = true;
-    }
+    static std::atomic<unsigned long long> done{0};
+    if (cudaError_t e = allow_shared(reinterpret_cast<const void*>(kern), C::SMEM, done)) return e;
     return launch_after(kern, dim3(a.parts, a.c.H * ((a.G + C::HEADS - 1) / C::HEADS), a.c.S), kWarps * 32, C::SMEM, s, a);
 }
 template <int D, bool F8> cudaError_t launch_width(const StepArgs& a, cudaStream_t s) {

@@ -207,7 +207,7 @@ def test_cache_object(dtype):
             c.write(layer, kv[:, 0].to(DEV), kv[:, 1].to(DEV), ch)
             at = 0
             for s, n in enumerate(counts):
-                text[layer][s] += list(held_as(kv[at:at + n], BF if dtype is BF else E4))
+                text[layer][s] += list(held_as(kv[at:at + n], dtype))
                 at += n
     chunk([20, 0, 15])
     chunk([10, 0, 1])
@@ -226,9 +226,8 @@ def test_cache_object(dtype):
                 if not text[layer][s]:
                     assert (out[s] == 0).all()
                     continue
-                text[layer][s].append(held_as(torch.stack([kn[s], vn[s]], 0).transpose(0, 1)[None], dtype)[0].transpose(0, 1).transpose(0, 1) if False else
-                                      held_as(torch.stack([kn[s], vn[s]], 1)[None], dtype)[0].transpose(0, 1))
-                r = torch.stack([t if t.shape[0] == 2 else t for t in text[layer][s]])           # [n,2,H,D]
+                text[layer][s].append(held_as(torch.stack([kn[s], vn[s]], 1)[None], dtype)[0].transpose(0, 1))
+                r = torch.stack(text[layer][s])                                                  # [n,2,H,D]
                 for h in range(H):
                     qs = q[s, h * G:(h + 1) * G].double()
                     o, spread, ds = attention64(qs, r[:, 0, h], r[:, 1, h], 1 / math.sqrt(D))
