@@ -404,8 +404,8 @@ int dsqg_ring_prefill(const void* k, const void* v, void* k_ring, void* v_ring,
 /* Root-mean-square norm of a residual stream, the addition in front of it included:
  *     h = x + residual (rounded to stream_dtype), y = h / sqrt(mean(h^2) + eps) * weight.
  * x, residual: bf16 or fp32 [rows,D], each its own type; residual nullable: h = x, which is not written.  y: bf16, fp32 or e4m3 with y_scale
- * [rows].  rstd [rows] fp32 (nullable): 1 / sqrt(..), for the backward pass.  Any D >= 1; rows start on 16 bytes and are read in pieces of eight
- * elements where D is a multiple of 8.  h may be residual or x where the types allow it. */
+ * [rows].  rstd [rows] fp32 (nullable): 1 / sqrt(..), for the backward pass.  Any D >= 1; tensors start on 16 bytes and are read in pieces of eight
+ * elements, of which two rows share one where D is no multiple of 8.  h may be residual or x where the types allow it. */
 typedef struct dsqg_rms_norm {
     const void* x; const void* residual; const float* weight;
     void* h; void* y; void* y_scale; float* rstd;
@@ -415,7 +415,7 @@ typedef struct dsqg_rms_norm {
 int dsqg_rms_norm_fwd(const dsqg_rms_norm* p, void* stream);
 /* Its backward pass for the gradients dy (y_dtype: bf16 or fp32) and dh (nullable, like h) of y and h:
  *     d = dh + rstd (w dy - x^ mean(w dy x^)), x^ = h rstd;  dx = d (x_dtype), dresidual = d (stream_dtype), dweight = sum over rows of dy x^.
- * Any of the three may be NULL.  Reads weight, rstd and h (x without a residual) of p.  The order of the sums follows from rows and D alone. */
+ * Any of the three may be NULL.  Reads weight, rstd and h (x without a residual) of p.  The order of the sums follows from rows, D and the types alone. */
 size_t dsqg_rms_norm_bwd_scratch_bytes(long long rows, int D);
 int dsqg_rms_norm_bwd(const dsqg_rms_norm* p, const void* dy, const void* dh, void* dx, void* dresidual, float* dweight, void* scratch, size_t scratch_bytes, void* stream);
 
