@@ -59,12 +59,12 @@ class Int4Linear(nn.Module):
         return m
 
     def _apply(self, fn, recurse=True):
-        # .to(dtype), .half(), ... move this module but leave its types alone: they are the format
-        types = {n: b.dtype for n, b in self._buffers.items() if b is not None}
+        # .to(dtype), .half(), ... move this module but leave its types and values alone: they are the format
+        before = dict(self._buffers)
         super()._apply(fn, recurse)
-        for n, dt in types.items():
-            if self._buffers[n].dtype != dt:
-                self._buffers[n] = self._buffers[n].to(dt)
+        for n, b in before.items():
+            if b is not None and self._buffers[n].dtype != b.dtype:
+                self._buffers[n] = b.to(self._buffers[n].device)
         return self
 
     def forward(self, x):

@@ -48,7 +48,7 @@ class PagedKVCache:
 
     kv [L,P,H,page,2,D] (`dtype` bf16, fp32 or float8_e4m3fn; then kv_scale [L,P,H,page,2] float8_e8m0fnu), block_table int32 [S,columns] and
     lengths int32 [S] are device tensors that never move, so a captured step replays on the lengths and pages of the day.  Which page
-    belongs to whom is kept on the host; `prefill`, `advance`, `reserve` and `release` are host calls, made outside a capture."""
+    belongs to whom is kept on the host; `extend`, `advance`, `reserve` and `release` are host calls, made outside a capture."""
 
     def __init__(self, layers, sequences, heads, head_dim, max_length, pages=None, page_size=64, dtype=torch.bfloat16, device="cuda"):
         if min(layers, sequences, heads, page_size, max_length) < 1:
@@ -100,7 +100,7 @@ class PagedKVCache:
             self.block_table.copy_(self._table)
 
     def release(self, sequence):
-        """Gives a sequence's pages back; its slot of the batch is empty (length 0) until the next prefill."""
+        """Gives a sequence's pages back; its slot of the batch is empty (length 0) until the next `extend`."""
         self._free.extend(reversed(self._owned[sequence]))
         self._owned[sequence] = []
         self._table[sequence] = -1

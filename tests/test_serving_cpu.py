@@ -170,3 +170,16 @@ def test_quantize_int4_packs_the_nearest_of_sixteen_values(group):
     n = dwarf_b200.Int4Linear(256, 5, group=group)
     n.load_state_dict(m.state_dict())
     assert torch.equal(n.weight, m.weight)
+
+
+def test_int4_linear_keeps_its_values_through_casts():
+    g = torch.Generator().manual_seed(0)
+    lin = torch.nn.Linear(64, 5)
+    with torch.no_grad():
+        lin.weight.copy_(torch.randn(5, 64, generator=g) * 1e6)
+        lin.bias.copy_(torch.randn(5, generator=g))
+    m = dwarf_b200.Int4Linear.from_linear(lin, 32)
+    before = {n: b.clone() for n, b in m.named_buffers()}
+    m.to(torch.bfloat16).half().float().double()
+    for n, b in m.named_buffers():
+        assert b.dtype == before[n].dtype and torch.equal(b, before[n])
