@@ -210,10 +210,10 @@ class CondMLM(nn.Module):
         t = state["t"]
         if t >= self.pos_embed.num_embeddings:
             raise ValueError("decode_token: position beyond the model's seq_len")
-        cache = state["cache"]
-        cache.advance()
         if "paged" in state:
             return self._decode_serving(ids_t, state)
+        cache = state["cache"]
+        cache.advance()
         x = self.embedding(ids_t) + self.pos_embed.weight[t]
         for i, blk in enumerate(self.blocks):
             h = blk.norm1(x)
@@ -230,7 +230,8 @@ class CondMLM(nn.Module):
     def _decode_serving(self, ids_t, state):
         t, cache, pages = state["t"], state["cache"], state["paged"]
         if pages is not None:
-            pages.advance()
+            pages.advance()                                     # raises, before anything has moved, when there is no room
+        cache.advance()
         x, branch = self.embedding(ids_t) + self.pos_embed.weight[t], None
         for i, blk in enumerate(self.blocks):
             full = i not in state["ring_of"]
