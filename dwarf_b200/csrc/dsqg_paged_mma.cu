@@ -13,7 +13,8 @@
 // 8 bits: e4m3 becomes f16 exactly.  Queries become f16 after a power of two that brings their largest element near 1; the keys' scales multiply the
 // scores; the values' scales multiply the probabilities, relative to the largest scale seen so far (another running maximum), so that f16 holds them.
 //
-// (Query heads as the 16 rows of the product instead: half of every accumulator idle up to 8 heads, 179 registers, 8 warps an SM and 636 instructions a
+// (Keys in 8 bits as they lie, through m16n8k32 with e4m3 operands and the query as two e4m3 numbers: 61 us instead of 58 for 4 sequences of 100001
+// positions.  Query heads as the 16 rows of the product instead: half of every accumulator idle up to 8 heads, 179 registers, 8 warps an SM and 636 instructions a
 // tile of 8-bit rows of 128 columns; 160 us for 4 sequences of 100001 positions, 4 x 8 heads.)
 //
 // mma.sync and not tcgen05: an operand of 128 rows would be at most an eighth full (query heads of one key-value head), and what is in question is memory.
@@ -225,8 +226,7 @@ __global__ void __launch_bounds__(kWarps * 32, CTAS) step_mma_kernel(const StepA
             __syncwarp();
         }
         // ---- scores: positions g and g + 8 of a tile, heads 2 t and 2 t + 1; two chains of products each, for they wait for one another
-        float sc[HT][4];
-        float odd[HT][4];
+        float sc[HT][4], odd[HT][4];
 #pragma unroll
         for (int n = 0; n < HT; ++n)
 #pragma unroll
@@ -236,7 +236,7 @@ __global__ void __launch_bounds__(kWarps * 32, CTAS) step_mma_kernel(const StepA
             uint32_t w[2][C::KB / 4];
             load_shared(st0 + C::at(g, (4 * k + t) * C::KB), w[0]);
             load_shared(st0 + C::at(g, (4 * k + t) * C::KB) + 8 * C::ROW, w[1]);      // s(g + 8) = s(g)
-            constexpr int N = F8 ? C::KB / 4 : 2;          // steps of a piece
+            constexpr int N = F8 ? C::KB / 4 : 2;              // steps of a piece
 #pragma unroll
             for (int e = 0; e < N; ++e) {
                 uint32_t ka[4];
@@ -260,14 +260,14 @@ __global__ void __launch_bounds__(kWarps * 32, CTAS) step_mma_kernel(const StepA
             bool nan = false;
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-                    uint16_t b;
-                    asm volatile("ld.shared.u16 %0, [%1];" : "=h"(b) : "r"(st0 + C::SOFF + 2 * (8 * j + g)) : "memory");
-                    if (!valid[j]) b = 0;
-                    kb[j] = b & 255u; vb[j] = b >> 8;
-                    nan |= kb[j] == 255u || vb[j] == 255u;
-                    top = max(top, vb[j]);
-                    ks[j] = __uint_as_float(kb[j] << 23);               // a byte of 0 (2^-127, which no row of this library has): 0
-                }
+                uint16_t b;
+                asm volatile("ld.shared.u16 %0, [%1];" : "=h"(b) : "r"(st0 + C::SOFF + 2 * (8 * j + g)) : "memory");
+                if (!valid[j]) b = 0;
+                kb[j] = b & 255u; vb[j] = b >> 8;
+                nan |= kb[j] == 255u || vb[j] == 255u;
+                top = max(top, vb[j]);
+                ks[j] = __uint_as_float(kb[j] << 23);              // a byte of 0 (2^-127, which no row of this library has): 0
+            }
             const bool some_nan = __any_sync(0xffffffffu, nan);
             if (some_nan) {
                 top = 0u;
@@ -287,12 +287,12 @@ __global__ void __launch_bounds__(kWarps * 32, CTAS) step_mma_kernel(const StepA
             }
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-                    vs[j] = relative_scale(vb[j], vtop);
-                    if (some_nan) {
-                        if (kb[j] == 255u) ks[j] = __uint_as_float(0x7fc00000u);
-                        if (vb[j] == 255u) vs[j] = __uint_as_float(0x7fc00000u);
-                    }
+                vs[j] = relative_scale(vb[j], vtop);
+                if (some_nan) {
+                    if (kb[j] == 255u) ks[j] = __uint_as_float(0x7fc00000u);
+                    if (vb[j] == 255u) vs[j] = __uint_as_float(0x7fc00000u);
                 }
+            }
         }
         uint32_t pb[HT][2];
 #pragma unroll
@@ -301,12 +301,12 @@ __global__ void __launch_bounds__(kWarps * 32, CTAS) step_mma_kernel(const StepA
 #pragma unroll
             for (int x = 0; x < 2; ++x)
 #pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-                        float& v = sc[n][2 * j + x];
-                        if constexpr (F8) v *= ks[j];
-                        v = valid[j] ? v : -INFINITY;
-                        mx[x] = fmaxf(mx[x], v);
-                    }
+                for (int j = 0; j < 2; ++j) {
+                    float& v = sc[n][2 * j + x];
+                    if constexpr (F8) v *= ks[j];
+                    v = valid[j] ? v : -INFINITY;
+                    mx[x] = fmaxf(mx[x], v);
+                }
             if (__any_sync(0xffffffffu, mx[0] > lim[n][0] || mx[1] > lim[n][1])) {
 #pragma unroll
                 for (int x = 0; x < 2; ++x) {
@@ -323,43 +323,43 @@ __global__ void __launch_bounds__(kWarps * 32, CTAS) step_mma_kernel(const StepA
             }
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-                    float x[2];
+                float x[2];
 #pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        x[e] = exp2_fast(fmaf(sc[n][2 * j + e], fs[n][e], -base[n][e]));
-                        l[n][e] += x[e];
-                        if constexpr (F8) x[e] *= vs[j];
-                    }
-                    // to 16 bits, as the operand of the product: relative 2^-9 (bf16) or 2^-12 (f16) on terms that add up, within the result's own rounding
-                    pb[n][j] = transposed(F8 ? pack_f16x2(x[0], x[1]) : pack_bf16x2(x[0], x[1]));
+                for (int e = 0; e < 2; ++e) {
+                    x[e] = exp2_fast(fmaf(sc[n][2 * j + e], fs[n][e], -base[n][e]));
+                    l[n][e] += x[e];
+                    if constexpr (F8) x[e] *= vs[j];
                 }
+                // to 16 bits, as the operand of the product: relative 2^-9 (bf16) or 2^-12 (f16) on terms that add up, within the result's own rounding
+                pb[n][j] = transposed(F8 ? pack_f16x2(x[0], x[1]) : pack_bf16x2(x[0], x[1]));
+            }
         }
         // ---- O^T += V^T P^T: rows g and g + 8 of m-tile (k VE + e) / 2 are d = 8 VE k + VE g + e and the next
 #pragma unroll
         for (int k = 0; k < C::VP; ++k) {
-                uint32_t w[4][C::VB / 4];
+            uint32_t w[4][C::VB / 4];
 #pragma unroll
-                for (int j = 0; j < 4; ++j)                    // positions 2 t, 2 t + 1 (+ 8)
-                    load_shared(st0 + C::at(2 * t + (j & 1), D * C::SZ + (8 * k + g) * C::VB) + 8 * (j >> 1) * C::ROW, w[j]);
+            for (int j = 0; j < 4; ++j)                    // positions 2 t, 2 t + 1 (+ 8)
+                load_shared(st0 + C::at(2 * t + (j & 1), D * C::SZ + (8 * k + g) * C::VB) + 8 * (j >> 1) * C::ROW, w[j]);
 #pragma unroll
-                for (int x = 0; x < C::VB / 4; ++x) {
-                    if constexpr (F8) {
+            for (int x = 0; x < C::VB / 4; ++x) {
+                if constexpr (F8) {
 #pragma unroll
-                        for (int y = 0; y < 2; ++y) {          // columns 2 y, 2 y + 1 of the word: {position, next position} of each
-                            uint32_t va[4];
-                            e4m3x4_half2(__byte_perm(w[0][x], w[1][x], y ? 0x7362 : 0x5140), va[0], va[1]);
-                            e4m3x4_half2(__byte_perm(w[2][x], w[3][x], y ? 0x7362 : 0x5140), va[2], va[3]);
+                    for (int y = 0; y < 2; ++y) {          // columns 2 y, 2 y + 1 of the word: {position, next position} of each
+                        uint32_t va[4];
+                        e4m3x4_half2(__byte_perm(w[0][x], w[1][x], y ? 0x7362 : 0x5140), va[0], va[1]);
+                        e4m3x4_half2(__byte_perm(w[2][x], w[3][x], y ? 0x7362 : 0x5140), va[2], va[3]);
 #pragma unroll
-                            for (int n = 0; n < HT; ++n) mma<true>(o[n][(k * C::VE + 4 * x) / 2 + y], va, pb[n][0], pb[n][1]);
-                        }
-                    } else {
-                        const uint32_t va[4] = {__byte_perm(w[0][x], w[1][x], 0x5410), __byte_perm(w[0][x], w[1][x], 0x7632),
-                                                __byte_perm(w[2][x], w[3][x], 0x5410), __byte_perm(w[2][x], w[3][x], 0x7632)};
-#pragma unroll
-                        for (int n = 0; n < HT; ++n) mma<false>(o[n][(k * C::VE + 2 * x) / 2], va, pb[n][0], pb[n][1]);
+                        for (int n = 0; n < HT; ++n) mma<true>(o[n][(k * C::VE + 4 * x) / 2 + y], va, pb[n][0], pb[n][1]);
                     }
+                } else {
+                    const uint32_t va[4] = {__byte_perm(w[0][x], w[1][x], 0x5410), __byte_perm(w[0][x], w[1][x], 0x7632),
+                                            __byte_perm(w[2][x], w[3][x], 0x5410), __byte_perm(w[2][x], w[3][x], 0x7632)};
+#pragma unroll
+                    for (int n = 0; n < HT; ++n) mma<false>(o[n][(k * C::VE + 2 * x) / 2], va, pb[n][0], pb[n][1]);
                 }
             }
+        }
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
     // ---- the four warps' results, joined in warp order
