@@ -73,7 +73,7 @@ __device__ __forceinline__ void new_row(const StepArgs& a, int s, int h, int pos
     }
 }
 
-// The tensor-core form (dsqg_paged_mma.cu): bf16 queries, pages in bf16 or e4m3, D a multiple of 32, pages of a multiple of 16 positions.
+// The tensor-core form (dsqg_paged_mma.cu): bf16 queries, pages in bf16 or e4m3, D 48, 80 or a multiple of 32, pages of a multiple of 16 positions.
 bool paged_mma_supported(const StepArgs& a);
 cudaError_t launch_paged_mma(const StepArgs& a, cudaStream_t s);
 

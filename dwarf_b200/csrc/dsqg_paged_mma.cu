@@ -1,4 +1,4 @@
-// One new token's attention to a paged cache on tensor cores: bf16 queries, pages in bf16 or e4m3, D = 32, 64, 96 or 128.
+// One new token's attention to a paged cache on tensor cores: bf16 queries, pages in bf16 or e4m3, D = 32, 48, 64, 80, 96 or 128.
 //
 // A block takes a part of one sequence for up to 8 HT query heads of one key-value head, a warp every fourth tile of 16 positions of it.  Positions are
 // the 16 rows of mma.sync (m16n8k16, fp32 accumulators) and the query heads its 8 columns: S^T = K Q^T, softmax with a running maximum and sum per
@@ -64,9 +64,12 @@ __device__ __forceinline__ uint32_t transposed(uint32_t x) {
 // 2^(byte - top) for a scale byte that is at most top
 __device__ __forceinline__ float relative_scale(uint32_t byte, uint32_t top) { return __uint_as_float((uint32_t)max(127 + (int)byte - (int)top, 0) << 23); }
 
-template <int D, bool F8, int HT, int STAGES>
+// DR: columns of the cache; D: of the products, DR rounded up to 32.  What is behind the DR columns of a key or value row is zero in shared memory, from the start on.
+template <int DR, bool F8, int HT, int STAGES>
 struct Cfg {
-    static constexpr int SZ = F8 ? 1 : 2, ROW = 2 * D * SZ;              // bytes of an element, of a position
+    static constexpr int D = (DR + 31) / 32 * 32;
+    static constexpr int SZ = F8 ? 1 : 2, ROW = 2 * D * SZ, HELD = 2 * DR * SZ;           // bytes of an element, of a position in shared memory and in the cache
+    static constexpr int PAD = (D - DR) * SZ / 16;                       // 16-byte pieces of zeros behind a row
     static constexpr int KB = F8 ? (D % 64 == 0 ? 16 : 8) : 16;          // bytes of a piece of a key row: four lanes take 4 KB bytes
     static constexpr int KP = D * SZ / (4 * KB);                         // pieces a lane and key row
     static constexpr int VB = F8 ? (D % 128 == 0 ? 16 : D % 64 == 0 ? 8 : 4) : (D % 64 == 0 ? 16 : 8);     // of a value row: eight lanes take 8 VB
@@ -77,9 +80,11 @@ struct Cfg {
     static constexpr int HEADS = 8 * HT;
     static constexpr int FIFO = kWarps * STAGES * STAGE, MERGE = kWarps * HEADS * (D + 2) * 4;
     static constexpr int BUF = FIFO > MERGE ? FIFO : MERGE;
-    static constexpr int SMEM = BUF + 2 * D * SZ + 16;
+    static constexpr int SMEM = BUF + HELD + 16;
     static constexpr int MT = D / 16;                                    // m-tiles of the output, and steps of the contraction over D
 
+    // A position's byte in the cache, in shared memory
+    __device__ static __forceinline__ int spread(int byte) { return PAD && byte >= DR * SZ ? byte + PAD * 16 : byte; }
     // Where a tile's byte `byte` of row `row` lies: pieces exchanged by s(row) in 0 .. 7.  The eight lanes of a read's phase ask for pieces x, .., x + 3 of two
     // neighbouring rows (keys: bit 2 of s tells them apart) or two pieces of four rows two apart (values: bits 1 and 2).
     __device__ static __forceinline__ int at(int row, int byte) {
@@ -88,12 +93,13 @@ struct Cfg {
 };
 
 // STAGES - 1 tiles of copies ahead.
-template <int D, bool F8, int HT, int STAGES, int CTAS>
+template <int DR, bool F8, int HT, int STAGES, int CTAS>
 __global__ void __launch_bounds__(kWarps * 32, CTAS) step_mma_kernel(const StepArgs a) {
-    using C = Cfg<D, F8, HT, STAGES>;
+    using C = Cfg<DR, F8, HT, STAGES>;
+    constexpr int D = C::D;
     extern __shared__ __align__(16) char smem[];
     char* const fresh = smem + C::BUF;
-    uint8_t* const fresh_scale = reinterpret_cast<uint8_t*>(fresh + 2 * D * C::SZ);
+    uint8_t* const fresh_scale = reinterpret_cast<uint8_t*>(fresh + C::HELD);
     stream_wait();
     const PageArgs& c = a.c;
     const int blocks_h = (a.G + C::HEADS - 1) / C::HEADS, hb = blockIdx.y % blocks_h, h = blockIdx.y / blocks_h, s = blockIdx.z, part = blockIdx.x;
@@ -124,6 +130,15 @@ __global__ void __launch_bounds__(kWarps * 32, CTAS) step_mma_kernel(const StepA
     const int tiles = r.end > first_tile ? (r.end - first_tile + STEP - 1) / STEP : 0;
     bool bad = r.bad;
 
+    if constexpr (C::PAD > 0) {
+        for (int z = lane; z < STAGES * kTile * 2 * C::PAD; z += 32) {
+            const int piece = z % C::PAD, half = z / C::PAD % 2, r = z / (2 * C::PAD) % kTile, stage = z / (2 * C::PAD * kTile);
+            const uint32_t to = fifo + stage * C::STAGE + C::at(r, half * D * C::SZ + DR * C::SZ + piece * 16);
+            asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" :: "r"(to), "r"(0) : "memory");
+        }
+        __syncwarp();
+    }
+
     // ---- copies
     const auto issue = [&](int i, uint32_t st) {
         const int id = next_id, row_in = next_row;
@@ -133,11 +148,11 @@ __global__ void __launch_bounds__(kWarps * 32, CTAS) step_mma_kernel(const StepA
             bad |= !there;
             const int n = there ? old_end - (first_tile + i * STEP) : 0;         // rows of the tile that exist
             const long long row0 = ((long long)(there ? id : 0) * c.H + h) * c.page + (there ? row_in : 0);
-            const char* const from = c.kv + row0 * C::ROW + lane * 16;
+            const char* const from = c.kv + row0 * C::HELD + lane * 16;
 #pragma unroll
-            for (int j = 0; j < kTile * C::ROW / 512; ++j) {
-                const int byte = j * 512 + lane * 16, r = byte / C::ROW;
-                copy_async<16>(st + C::at(r, byte % C::ROW), from + j * 512, r < n);
+            for (int j = 0; j < kTile * C::HELD / 512; ++j) {
+                const int byte = j * 512 + lane * 16, r = byte / C::HELD;
+                copy_async<16>(st + C::at(r, C::spread(byte % C::HELD)), from + j * 512, r < n);
             }
             if constexpr (F8)
                 if (lane < kTile / 2) copy_async<4>(st + C::SOFF + lane * 4, reinterpret_cast<const char*>(c.scale) + row0 * 2 + lane * 4, true);
@@ -154,7 +169,7 @@ __global__ void __launch_bounds__(kWarps * 32, CTAS) step_mma_kernel(const StepA
     uint32_t qb[HT][C::MT][2];
     float fs[HT][2];                                           // what the scores of columns 2 t, 2 t + 1 are multiplied by
     {
-        const __nv_bfloat16* q = static_cast<const __nv_bfloat16*>(a.q) + q0 * D;
+        const __nv_bfloat16* q = static_cast<const __nv_bfloat16*>(a.q) + q0 * DR;
         constexpr int E = C::KB / C::SZ;                       // elements of a piece: E / 4 steps
 #pragma unroll
         for (int n = 0; n < HT; ++n) {
@@ -164,7 +179,7 @@ __global__ void __launch_bounds__(kWarps * 32, CTAS) step_mma_kernel(const StepA
 #pragma unroll
                 for (int e = 0; e < E / 4; ++e) {
                     uint2 u = make_uint2(0u, 0u);
-                    if (on) u = *reinterpret_cast<const uint2*>(q + (g + 8 * n) * D + (4 * k + t) * E + 4 * e);
+                    if (on && (4 * k + t) * E + 4 * e < DR) u = *reinterpret_cast<const uint2*>(q + (g + 8 * n) * DR + (4 * k + t) * E + 4 * e);
                     qb[n][k * (E / 4) + e][0] = u.x; qb[n][k * (E / 4) + e][1] = u.y;
                 }
             fs[n][0] = fs[n][1] = a.scale;
@@ -221,7 +236,7 @@ __global__ void __launch_bounds__(kWarps * 32, CTAS) step_mma_kernel(const StepA
         if (last >= p0 && last < p0 + kTile) {                 // the new token's row: from where new_row left it
             const int key = last - p0;
             char* const to = smem + (st0 - static_cast<uint32_t>(__cvta_generic_to_shared(smem)));
-            if (lane * 16 < C::ROW) *reinterpret_cast<uint4*>(to + C::at(key, lane * 16)) = *reinterpret_cast<const uint4*>(fresh + lane * 16);
+            if (lane * 16 < C::HELD) *reinterpret_cast<uint4*>(to + C::at(key, C::spread(lane * 16))) = *reinterpret_cast<const uint4*>(fresh + lane * 16);
             if (F8 && lane < 2) to[C::SOFF + 2 * key + lane] = fresh_scale[lane];
             __syncwarp();
         }
@@ -381,8 +396,8 @@ __global__ void __launch_bounds__(kWarps * 32, CTAS) step_mma_kernel(const StepA
                 for (int e = 0; e < C::VE; ++e) so[at * D + 8 * C::VE * k + C::VE * g + e] = o[n][(k * C::VE + e) / 2][2 * (e & 1) + x] * unit;
         }
     __syncthreads();
-    for (int z = threadIdx.x; z < heads * D; z += kWarps * 32) {
-        const int row = z / D, d = z - row * D;
+    for (int z = threadIdx.x; z < heads * DR; z += kWarps * 32) {
+        const int row = z / DR, d = z - row * DR;
         float M = -INFINITY;
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) M = fmaxf(M, sml[(w * C::HEADS + row) * 2]);
@@ -397,8 +412,8 @@ __global__ void __launch_bounds__(kWarps * 32, CTAS) step_mma_kernel(const StepA
         if (a.ml) {
             const long long at = (q0 + row) * a.parts + part;
             if (d == 0) a.ml[at] = make_float2(M, L);
-            a.acc[at * D + d] = A;
-        } else static_cast<__nv_bfloat16*>(a.out)[(q0 + row) * D + d] = __float2bfloat16(L == 0.f ? 0.f : A / L);
+            a.acc[at * DR + d] = A;
+        } else static_cast<__nv_bfloat16*>(a.out)[(q0 + row) * DR + d] = __float2bfloat16(L == 0.f ? 0.f : A / L);
     }
 }
 
@@ -419,7 +434,9 @@ template <int D, bool F8> cudaError_t launch_width(const StepArgs& a, cudaStream
 template <bool F8> cudaError_t launch_type(const StepArgs& a, cudaStream_t s) {
     switch (a.c.D) {
         case 32: return launch_width<32, F8>(a, s);
+        case 48: return launch_width<48, F8>(a, s);
         case 64: return launch_width<64, F8>(a, s);
+        case 80: return launch_width<80, F8>(a, s);
         case 96: return launch_width<96, F8>(a, s);
         default: return launch_width<128, F8>(a, s);
     }
@@ -428,7 +445,7 @@ template <bool F8> cudaError_t launch_type(const StepArgs& a, cudaStream_t s) {
 }  // namespace
 
 bool paged_mma_supported(const StepArgs& a) {
-    return !a.q_f32 && (a.c.dtype == DSQG_DTYPE_BF16 || a.c.dtype == DSQG_DTYPE_E4M3) && a.c.D % 32 == 0 && a.c.page % kTile == 0 &&
+    return !a.q_f32 && (a.c.dtype == DSQG_DTYPE_BF16 || a.c.dtype == DSQG_DTYPE_E4M3) && (a.c.D % 32 == 0 || a.c.D == 48 || a.c.D == 80) && a.c.page % kTile == 0 &&
            (reinterpret_cast<uintptr_t>(a.c.scale) & 3u) == 0;
 }
 cudaError_t launch_paged_mma(const StepArgs& a, cudaStream_t s) { return a.c.dtype == DSQG_DTYPE_E4M3 ? launch_type<true>(a, s) : launch_type<false>(a, s); }

@@ -64,7 +64,8 @@ def check_step(lengths, H, G, D, page, dtype, q_dt, new=True, max_length=None, s
     out = dwarf_b200.paged_attention_step(q.to(DEV), *args, kv, table, ln, kv_scale=ks, scale=scale, max_length=max_length)
     assert out.shape == q.shape and out.dtype is q_dt
     sc = 1 / math.sqrt(D) if scale is None else scale
-    p_half = 0.0 if (q_dt is F or dtype is F or D % 32 or page % 16) else 2.0 ** -8 if dtype is BF else 2.0 ** -11      # probabilities as an operand in 16 bits
+    # the form on tensor cores: widths that are multiples of 32, and 48 and 80, pages of a multiple of 16 positions
+    p_half = 0.0 if (q_dt is F or dtype is F or (D % 32 and D not in (48, 80)) or page % 16) else 2.0 ** -8 if dtype is BF else 2.0 ** -11      # probabilities as an operand in 16 bits
     for s, n in enumerate(lengths):
         for h in range(H):
             r = rows[s][:, h].clone()
@@ -98,7 +99,7 @@ TYPES = [(BF, BF), (E4, BF), (F, F), (E4, F), (BF, F), (F, BF)]
 
 @pytest.mark.parametrize("dtype,q_dt", TYPES, ids=lambda t: str(t).split(".")[-1])
 @pytest.mark.parametrize("H,G,D,page", [(1, 1, 32, 16), (2, 1, 64, 48), (1, 4, 128, 64), (2, 3, 96, 16), (1, 12, 64, 32), (1, 20, 32, 16), (2, 2, 80, 16), (1, 1, 8, 16),
-                                        (1, 5, 64, 10), (2, 1, 40, 1), (1, 17, 128, 16), (3, 8, 128, 32)])
+                                        (1, 5, 64, 10), (2, 1, 40, 1), (1, 17, 128, 16), (3, 8, 128, 32), (2, 3, 48, 16), (1, 9, 80, 48), (1, 17, 48, 64), (3, 8, 80, 32)])
 def test_step(dtype, q_dt, H, G, D, page):
     check_step([0, 1, 2, 15, 16, 17, 63, 64, 65, 130], H, G, D, page, dtype, q_dt)
     check_step([33, 16], H, G, D, page, dtype, q_dt, new=False, scale=0.3)
@@ -109,6 +110,7 @@ def test_step(dtype, q_dt, H, G, D, page):
 def test_step_split_over_the_length(dtype, q_dt, lengths, most):
     check_step(lengths, 2, 2, 64, 64, dtype, q_dt, max_length=most)
     check_step(lengths, 1, 1, 40, 20, dtype, q_dt, max_length=most)
+    check_step(lengths, 1, 3, 80, 32, dtype, q_dt, max_length=most)
 
 
 def test_bad_tables_and_lengths_give_nan_and_touch_nothing():
