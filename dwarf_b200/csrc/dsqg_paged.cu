@@ -158,9 +158,9 @@ template <bool WRITE> cudaError_t launch_move_heads(const MoveArgs& a, cudaStrea
 // ---- attention of one new token, CUDA cores: fp32 arithmetic for any types, D a multiple of 8 up to 128, pages of any length.
 // A block takes a part of one sequence for up to four query heads of one key-value head; a group of LPR lanes takes a position at a time and
 // keeps the running maximum and sum of its softmax for each of those heads; the groups are joined in shared memory in a fixed order.
-constexpr int kStepThreads = 128, kHeads = 4;
+constexpr int kStepThreads = 128;
 
-template <int LPR>
+template <int LPR, int kHeads>
 __global__ void __launch_bounds__(kStepThreads) step_kernel(const StepArgs a) {
     __shared__ __align__(16) char fresh[2 * 128 * 4];
     __shared__ uint8_t fresh_scale[2];
@@ -188,27 +188,36 @@ __global__ void __launch_bounds__(kStepThreads) step_kernel(const StepArgs a) {
     }
     bool bad = r.bad;
     const int last = has_new ? r.length - 1 : -1;
-    for (int p0 = r.first; p0 < r.end; p0 += kStepThreads / LPR) {
-        const int p = p0 + group;
-        float k[8] = {0, 0, 0, 0, 0, 0, 0, 0}, v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-        bool valid = p < r.end;
-        if (valid) {
-            const long long first = c.rows_of(s, h, p / c.page);
-            if (first < 0) { bad = true; valid = false; }
-            else if (on) {
-                const long long slot = (first + p % c.page) * 2;
-                const bool is_new = p == last;
-                const void* rows = is_new ? static_cast<const void*>(fresh) : c.kv;
-                load8_as(rows, is_new ? d : slot * D + d, c.dtype, k);
-                load8_as(rows, is_new ? D + d : (slot + 1) * D + d, c.dtype, v);
-                if (c.dtype == DSQG_DTYPE_E4M3) {
-                    const uint8_t* b = is_new ? fresh_scale : c.scale + slot;
-                    const float sk = scale_value(b[0]), sv = scale_value(b[1]);
+    struct Row { float k[8], v[8]; bool valid; };
+    const auto fetch = [&](int p) {
+        Row x;
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) { k[e] *= sk; v[e] *= sv; }
-                }
-            }
+        for (int e = 0; e < 8; ++e) x.k[e] = x.v[e] = 0.f;
+        x.valid = p < r.end;
+        if (!x.valid) return x;
+        const long long first = c.rows_of(s, h, p / c.page);
+        if (first < 0) { bad = true; x.valid = false; return x; }
+        if (!on) return x;
+        const long long slot = (first + p % c.page) * 2;
+        const bool is_new = p == last;
+        const void* rows = is_new ? static_cast<const void*>(fresh) : c.kv;
+        load8_as(rows, is_new ? d : slot * D + d, c.dtype, x.k);
+        load8_as(rows, is_new ? D + d : (slot + 1) * D + d, c.dtype, x.v);
+        if (c.dtype == DSQG_DTYPE_E4M3) {
+            const uint8_t* b = is_new ? fresh_scale : c.scale + slot;
+            const float sk = scale_value(b[0]), sv = scale_value(b[1]);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) { x.k[e] *= sk; x.v[e] *= sv; }
         }
+        return x;
+    };
+    constexpr int STEP = kStepThreads / LPR;
+    Row next = fetch(r.first + group);
+    for (int p0 = r.first; p0 < r.end; p0 += STEP) {
+        const Row now = next;
+        next = fetch(p0 + STEP + group);                       // on its way while this one is used
+        const float (&k)[8] = now.k, (&v)[8] = now.v;
+        const bool valid = now.valid;
 #pragma unroll
         for (int i = 0; i < kHeads; ++i) {
             float dot = 0.f;
@@ -330,14 +339,18 @@ cudaError_t launch_join(const StepArgs& a, cudaStream_t s) {
     return launch_after(join_kernel<8>, grid(8), kJoinWarps * 32, 0, s, a);
 }
 
+// One query head a block where a key-value head has one, else up to four.
+template <int LPR> cudaError_t launch_lanes(const StepArgs& a, cudaStream_t s) {
+    if (a.G == 1) return launch_after(step_kernel<LPR, 1>, dim3(a.parts, a.c.H, a.c.S), kStepThreads, 0, s, a);
+    return launch_after(step_kernel<LPR, 4>, dim3(a.parts, a.c.H * ((a.G + 3) / 4), a.c.S), kStepThreads, 0, s, a);
+}
 cudaError_t launch_step(const StepArgs& a, cudaStream_t s) {
     const int lanes = a.c.D / 8;
-    const dim3 grid(a.parts, a.c.H * ((a.G + kHeads - 1) / kHeads), a.c.S);
-    if (lanes <= 1) return launch_after(step_kernel<1>, grid, kStepThreads, 0, s, a);
-    if (lanes <= 2) return launch_after(step_kernel<2>, grid, kStepThreads, 0, s, a);
-    if (lanes <= 4) return launch_after(step_kernel<4>, grid, kStepThreads, 0, s, a);
-    if (lanes <= 8) return launch_after(step_kernel<8>, grid, kStepThreads, 0, s, a);
-    return launch_after(step_kernel<16>, grid, kStepThreads, 0, s, a);
+    if (lanes <= 1) return launch_lanes<1>(a, s);
+    if (lanes <= 2) return launch_lanes<2>(a, s);
+    if (lanes <= 4) return launch_lanes<4>(a, s);
+    if (lanes <= 8) return launch_lanes<8>(a, s);
+    return launch_lanes<16>(a, s);
 }
 
 inline bool bad(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) != 0; }
