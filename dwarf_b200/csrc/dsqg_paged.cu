@@ -157,7 +157,9 @@ template <bool WRITE> cudaError_t launch_move_heads(const MoveArgs& a, cudaStrea
 
 // ---- attention of one new token, CUDA cores: fp32 arithmetic for any types, D a multiple of 8 up to 128, pages of any length.
 // A block takes a part of one sequence for up to four query heads of one key-value head; a group of LPR lanes takes a position at a time and
-// keeps the running maximum and sum of its softmax for each of those heads; the groups are joined in shared memory in a fixed order.
+// keeps the running maximum and sum of its softmax for each of those heads, the next position on its way; the groups are joined in shared memory in a
+// fixed order.  Bound by its instructions: a dot product over LPR lanes by shuffles for every position and head.  16 sequences up to 2048, 8 heads of 64
+// in fp32: 20.5 us (four heads a block, three of them idle, and nothing asked for ahead: 32.1; memory's floor 8.6); 64 up to 4096, 8 x 4 heads of 128: 409 (170).
 constexpr int kStepThreads = 128;
 
 template <int LPR, int kHeads>
@@ -267,7 +269,8 @@ __global__ void __launch_bounds__(kStepThreads) step_kernel(const StepArgs a) {
 }
 
 // Joins the parts of a sequence: W warps per (sequence, query head), four parts a warp at a time (maximum, sum and values asked for together), the warps
-// added in order.  What it waits for is memory: W so that no warp goes round twice up to 32 parts, and not more, for there may be many rows of few parts.
+// added in order.  What it waits for is memory: W so that no warp goes round twice up to 32 parts, and not more, for there may be many rows of few parts
+// (2048 rows of two parts: 6 us with one warp each, 13 with eight).
 // (One warp per row, parts one after the other: 40 us for 128 rows of 98 parts, which is a chain of loads.)
 constexpr int kJoinWarps = 8;
 template <int W> __global__ void __launch_bounds__(kJoinWarps * 32) join_kernel(const StepArgs a) {
