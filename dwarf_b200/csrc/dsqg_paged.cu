@@ -360,13 +360,15 @@ inline bool bad(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) !
 
 // The positions of a part: a multiple of 64, from the sizes alone.  Of blocks that run at once (`an_sm` per SM) about 85 % shall have work if lengths are spread
 // evenly up to the longest: below all of them, for one block too many takes as long as twice as many.  From 16 sequences on, which differ more, twice as many
-// parts.  Up to 2048 positions a part.  (us, with one part of the longest for every block that runs at once, whatever the lengths / with this: 16 sequences
-// up to 8192, 8 x 4 heads of 128 in 8 bits, 44 / 34; 4 up to 20000, 4 x 8 heads in 8 bits, 21.7 / 19.1; one of 4096, 8 x 4 heads in bf16, 10.5 / 7.6.)
+// parts.  Up to 2048 positions a part, up to 3200 where all blocks then run at once (55.4 us instead of 58.1 for 4 up to 100001, 4 x 8 heads in 8 bits; parts of
+// 2048 would be 564 blocks for 444 places: 64.8).  (us, with one part of the longest for every block that runs at once, whatever the lengths / with this: 16 sequences
+// up to 8192, 8 x 4 heads of 128 in 8 bits, 44 / 33; 4 up to 20000, 4 x 8 heads in 8 bits, 21.7 / 17.6; one of 4096, 8 x 4 heads in bf16, 10.5 / 7.6.)
 struct Split { int chunk, parts; };
 inline Split split_for(int S, int H, int G, int limit, int an_sm) {
     const double pairs = (double)S * H * ((G + 15) / 16), share = (S + 1) / (2.0 * S), blocks = 148 * an_sm * 0.85 * (S < 16 ? 1 : 2);
     const long long most = ((long long)limit + 63) / 64;                       // in units of 64 positions
-    long long units = (long long)std::ceil(std::min(pairs * most * share / blocks, 32.0));
+    const double even = pairs * most * share / blocks;
+    long long units = (long long)std::ceil(S < 16 && even <= 50 ? even : std::min(even, 32.0));
     const long long least = (most + 1023) / 1024;                              // no more than 1024 parts
     if (units < least) units = least;
     if (units < 1) units = 1;
@@ -377,7 +379,7 @@ inline Split split_for(int S, int H, int G, int limit, int an_sm) {
     return r;
 }
 // Blocks of the kernel that a step takes that an SM holds.
-inline int blocks_an_sm(bool mma, int G, bool f8) { return mma && (G > 8 || !f8) ? 2 : 4; }
+inline int blocks_an_sm(bool mma, int G, int D, bool f8) { return !mma ? 4 : G > 8 || !f8 ? 2 : D > 96 ? 3 : 4; }
 
 // A description of a cache that kernels may use.
 int page_args(const dsqg_pages* c, PageArgs* a) {
@@ -428,7 +430,8 @@ int dsqg_paged_read(const dsqg_pages* cache, void* k, void* v, const int32_t* cu
 
 size_t dsqg_paged_step_scratch_bytes(int sequences, int heads, int q_heads, int D, int max_length) {
     if (sequences < 1 || heads < 1 || q_heads < heads || q_heads % heads || D < 1 || max_length < 0) return 0;
-    const int parts = std::max(split_for(sequences, heads, q_heads / heads, max_length, 2).parts, split_for(sequences, heads, q_heads / heads, max_length, 4).parts);
+    int parts = 1;                                             // whatever the types
+    for (int n = 2; n <= 4; ++n) parts = std::max(parts, split_for(sequences, heads, q_heads / heads, max_length, n).parts);
     return parts == 1 ? 0 : (size_t)sequences * q_heads * parts * (D + 2) * 4;
 }
 
@@ -446,7 +449,7 @@ int dsqg_paged_step(const dsqg_pages* cache, const void* q, const void* k_new, c
     a.q = q; a.k_new = k_new; a.v_new = v_new; a.lengths = lengths; a.out = out; a.G = q_heads / a.c.H; a.q_f32 = dtype == DSQG_DTYPE_F32;
     a.scale = (scale > 0.f ? scale : 1.0f / sqrtf((float)a.c.D)) * 1.4426950408889634f;
     const bool mma = paged_mma_supported(a);
-    const Split p = split_for(a.c.S, a.c.H, a.G, a.limit, blocks_an_sm(mma, a.G, a.c.dtype == DSQG_DTYPE_E4M3));
+    const Split p = split_for(a.c.S, a.c.H, a.G, a.limit, blocks_an_sm(mma, a.G, a.c.D, a.c.dtype == DSQG_DTYPE_E4M3));
     a.chunk = p.chunk; a.parts = p.parts; a.ml = nullptr; a.acc = nullptr;
     if (p.parts > 1) {
         const size_t rows = (size_t)a.c.S * q_heads * p.parts;

@@ -425,11 +425,12 @@ template <int D, bool F8, int HT, int STAGES, int CTAS> cudaError_t launch_one(c
     return launch_after(kern, dim3(a.parts, a.c.H * ((a.G + C::HEADS - 1) / C::HEADS), a.c.S), kWarps * 32, C::SMEM, s, a);
 }
 template <int D, bool F8> cudaError_t launch_width(const StepArgs& a, cudaStream_t s) {
-    // Two CTAs of four warps and 8-KB tiles in bf16, four in 8 bits, two tiles ahead each: 87 us for 64 sequences up to 4096, 8 x 4 heads of 128 in bf16 (84 at
-    // the rate of a copy), 58 us for 4 up to 100001, 4 x 8 heads of 128 in 8 bits (44).  Three CTAs and one tile ahead cost 1 % and 14 % more, two tiles a round
-    // with three CTAs 14 % in 8 bits; tiles by the copy engine through a swizzled tensor map 2 % more in bf16 and 2 % less in 8 bits.
+    // Two CTAs of four warps and 8-KB tiles in bf16, three in 8 bits, four up to 96 columns, two tiles ahead each: 87 us for 64 sequences up to 4096, 8 x 4 heads
+    // of 128 in bf16 (84 at the rate of a copy), 55.4 us for 4 up to 100001, 4 x 8 heads of 128 in 8 bits (44).  Four CTAs in 8 bits: 17.7 -> 19.0 for 4 up to 20000,
+    // 33.1 -> 33.9 for 16 up to 8192; three at 80 columns 31.7 -> 32.7.  Three tiles ahead: the same.  bf16 with three CTAs and one tile ahead 1 % more, two tiles
+    // a round 14 % more in 8 bits; tiles by the copy engine through a swizzled tensor map 2 % more in bf16 and 2 % less in 8 bits.
     if (a.G > 8) return launch_one<D, F8, 2, 3, 2>(a, s);
-    return launch_one<D, F8, 1, 3, F8 ? 4 : 2>(a, s);
+    return launch_one<D, F8, 1, 3, (!F8 ? 2 : D > 96 ? 3 : 4)>(a, s);
 }
 template <bool F8> cudaError_t launch_type(const StepArgs& a, cudaStream_t s) {
     switch (a.c.D) {
