@@ -309,7 +309,7 @@ __global__ void __launch_bounds__(kWarps * 32, CTAS) step_mma_kernel(const StepA
                 }
             }
         }
-        uint32_t pb[HT][2];
+        uint32_t pb[HT][2], pl[HT][2];                         // P^T in two numbers of 16 bits
 #pragma unroll
         for (int n = 0; n < HT; ++n) {
             float mx[2] = {-INFINITY, -INFINITY};
@@ -345,8 +345,14 @@ __global__ void __launch_bounds__(kWarps * 32, CTAS) step_mma_kernel(const StepA
                     l[n][e] += x[e];
                     if constexpr (F8) x[e] *= vs[j];
                 }
-                // to 16 bits, as the operand of the product: relative 2^-9 (bf16) or 2^-12 (f16) on terms that add up, within the result's own rounding
-                pb[n][j] = transposed(F8 ? pack_f16x2(x[0], x[1]) : pack_bf16x2(x[0], x[1]));
+                if constexpr (F8) pb[n][j] = transposed(pack_f16x2(x[0], x[1]));      // relative 2^-11 on terms that add up
+                else {
+                    // two operands in bf16, the number and what its rounding left: together off by 2^-16 of it.  One alone (2^-8) is seen in the result: 0.0023
+                    // from 64 bits (2-norms, 64 sequences up to 4096, 8 x 4 heads of 128), where the result's own rounding to bf16 is 0.0017.
+                    const uint32_t hi = pack_bf16x2(x[0], x[1]);
+                    pb[n][j] = transposed(hi);
+                    pl[n][j] = transposed(pack_bf16x2(x[0] - __uint_as_float(hi << 16), x[1] - __uint_as_float(hi & 0xffff0000u)));
+                }
             }
         }
         // ---- O^T += V^T P^T: rows g and g + 8 of m-tile (k VE + e) / 2 are d = 8 VE k + VE g + e and the next
@@ -371,7 +377,10 @@ __global__ void __launch_bounds__(kWarps * 32, CTAS) step_mma_kernel(const StepA
                     const uint32_t va[4] = {__byte_perm(w[0][x], w[1][x], 0x5410), __byte_perm(w[0][x], w[1][x], 0x7632),
                                             __byte_perm(w[2][x], w[3][x], 0x5410), __byte_perm(w[2][x], w[3][x], 0x7632)};
 #pragma unroll
-                    for (int n = 0; n < HT; ++n) mma<false>(o[n][(k * C::VE + 2 * x) / 2], va, pb[n][0], pb[n][1]);
+                    for (int n = 0; n < HT; ++n) {
+                        mma<false>(o[n][(k * C::VE + 2 * x) / 2], va, pb[n][0], pb[n][1]);
+                        mma<false>(o[n][(k * C::VE + 2 * x) / 2], va, pl[n][0], pl[n][1]);
+                    }
                 }
             }
         }
@@ -425,7 +434,7 @@ template <int D, bool F8, int HT, int STAGES, int CTAS> cudaError_t launch_one(c
     return launch_after(kern, dim3(a.parts, a.c.H * ((a.G + C::HEADS - 1) / C::HEADS), a.c.S), kWarps * 32, C::SMEM, s, a);
 }
 template <int D, bool F8> cudaError_t launch_width(const StepArgs& a, cudaStream_t s) {
-    // Two CTAs of four warps and 8-KB tiles in bf16, three in 8 bits, four up to 96 columns, two tiles ahead each: 87 us for 64 sequences up to 4096, 8 x 4 heads
+    // Two CTAs of four warps and 8-KB tiles in bf16, three in 8 bits, four up to 96 columns, two tiles ahead each: 88 us for 64 sequences up to 4096, 8 x 4 heads
     // of 128 in bf16 (84 at the rate of a copy), 55.4 us for 4 up to 100001, 4 x 8 heads of 128 in 8 bits (44).  Four CTAs in 8 bits: 17.7 -> 19.0 for 4 up to 20000,
     // 33.1 -> 33.9 for 16 up to 8192; three at 80 columns 31.7 -> 32.7.  Three tiles ahead: the same.  bf16 with three CTAs and one tile ahead 1 % more, two tiles
     // a round 14 % more in 8 bits; tiles by the copy engine through a swizzled tensor map 2 % more in bf16 and 2 % less in 8 bits.
