@@ -11,7 +11,9 @@
 // P^T turns from a result into an operand by movmatrix.
 //
 // 8 bits: e4m3 becomes f16 exactly.  Queries become f16 after a power of two that brings their largest element near 1; the keys' scales multiply the
-// scores; the values' scales multiply the probabilities, relative to the largest scale seen so far (another running maximum), so that f16 holds them.
+// scores; the values' scales multiply the probabilities, as exponents: an operand is 2^(score + exponent of its value row's scale - w), w a running base of
+// each column that follows the largest of these sums, so that what is largest in the result is largest in f16, whatever scales other rows have.  (Relative to the
+// largest scale alone, a value row 2^20 above the others took the bits of all that came with or after it, even one that no query looks at.)
 //
 // (Keys in 8 bits as they lie, through m16n8k32 with e4m3 operands and the query as two e4m3 numbers: 61 us instead of 58 for 4 sequences of 100001
 // positions.  Query heads as the 16 rows of the product instead: half of every accumulator idle up to 8 heads, 179 registers, 8 warps an SM and 636 instructions a
@@ -28,6 +30,9 @@ constexpr int kWarps = 4, kTile = 16;
 // f16, bf16 and the fp32 sums hold as well as those below 1.  A warp then rescales once or twice; at every new maximum of any of eight heads it did so at
 // 13 of its first 16 tiles.
 constexpr float kSlack = 8.f;
+// The operands of 8-bit pages: rescaled when one would be above 2^15 (f16 ends at 65504), the largest then to about 2^10.  Two f16 numbers hold 2^-22 of an
+// operand from 2^-3 on, and 2^-25 below: 2^-34.5 of the largest since the last rescaling, times the 2 that maxima of e4m3 rows are apart.
+constexpr float kTop = 15.f, kLevel = 10.f;
 
 template <bool F16> __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     if constexpr (F16)
@@ -61,8 +66,8 @@ __device__ __forceinline__ uint32_t transposed(uint32_t x) {
     asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
     return y;
 }
-// 2^(byte - top) for a scale byte that is at most top
-__device__ __forceinline__ float relative_scale(uint32_t byte, uint32_t top) { return __uint_as_float((uint32_t)max(127 + (int)byte - (int)top, 0) << 23); }
+// log2 of the scale that a byte stands for
+__device__ __forceinline__ float log2_scale(uint32_t byte) { return __uint_as_float(0x4b000000u | byte) - 8388735.f; }
 
 // DR: columns of the cache; D: of the products, DR rounded up to 32.  What is behind the DR columns of a key or value row is zero in shared memory, from the start on.
 template <int DR, bool F8, int HT, int STAGES>
@@ -193,7 +198,8 @@ __global__ void __launch_bounds__(kWarps * 32, CTAS) step_mma_kernel(const StepA
                 // largest element to [1, 2): nothing is lost but what is below 2^-25 of it.  NaN and infinity stay what they are.
                 int ex = (int)(top >> 23);
                 ex = ex == 0 ? 127 : ex >= 254 ? 253 : ex;
-                const float down = __uint_as_float((254u - ex) << 23), up = a.scale * __uint_as_float((uint32_t)ex << 23);
+                // not 0, for what is masked is -inf times it
+                const float down = __uint_as_float((254u - ex) << 23), up = fmaxf(a.scale * __uint_as_float((uint32_t)ex << 23), 1.17549435e-38f);
 #pragma unroll
                 for (int k = 0; k < C::MT; ++k)
 #pragma unroll
@@ -212,16 +218,15 @@ __global__ void __launch_bounds__(kWarps * 32, CTAS) step_mma_kernel(const StepA
 
     float o[HT][C::MT][4];
     // m: what the exponentials are taken against, at least the running maximum less kSlack / fs; base: m fs, 0 where m is still -inf
-    float m[HT][2], l[HT][2], base[HT][2], lim[HT][2];
+    float m[HT][2], l[HT][2], base[HT][2], lim[HT][2], wbase[HT][2];          // wbase: w above, a whole number
 #pragma unroll
     for (int n = 0; n < HT; ++n) {
 #pragma unroll
         for (int k = 0; k < C::MT; ++k)
 #pragma unroll
             for (int e = 0; e < 4; ++e) o[n][k][e] = 0.f;
-        m[n][0] = m[n][1] = lim[n][0] = lim[n][1] = -INFINITY; l[n][0] = l[n][1] = base[n][0] = base[n][1] = 0.f;
+        m[n][0] = m[n][1] = lim[n][0] = lim[n][1] = -INFINITY; l[n][0] = l[n][1] = base[n][0] = base[n][1] = 0.f; wbase[n][0] = wbase[n][1] = -1e30f;
     }
-    uint32_t vtop = 0u;                                        // largest scale byte of a value row so far
     int slot = 0;
 
 #pragma unroll 1
@@ -267,11 +272,11 @@ __global__ void __launch_bounds__(kWarps * 32, CTAS) step_mma_kernel(const StepA
             for (int e = 0; e < 4; ++e) sc[n][e] += odd[n][e];
         // ---- softmax.  A score is the product times its row's scale (ks), in units of 1 / fs; m is in the same units.
         bool valid[2];
-        float ks[2], vs[2];
+        float ks[2], vlog[2];                                  // vlog: log2 of the value rows' scales
 #pragma unroll
-        for (int j = 0; j < 2; ++j) { valid[j] = p0 + 8 * j + g < r.end; ks[j] = vs[j] = 1.f; }
+        for (int j = 0; j < 2; ++j) { valid[j] = p0 + 8 * j + g < r.end; ks[j] = 1.f; vlog[j] = 0.f; }
         if constexpr (F8) {
-            uint32_t kb[2], vb[2], top = 0u;
+            uint32_t kb[2], vb[2];
             bool nan = false;
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
@@ -280,32 +285,14 @@ __global__ void __launch_bounds__(kWarps * 32, CTAS) step_mma_kernel(const StepA
                 if (!valid[j]) b = 0;
                 kb[j] = b & 255u; vb[j] = b >> 8;
                 nan |= kb[j] == 255u || vb[j] == 255u;
-                top = max(top, vb[j]);
                 ks[j] = __uint_as_float(kb[j] << 23);              // a byte of 0 (2^-127, which no row of this library has): 0
+                vlog[j] = log2_scale(vb[j]);
             }
-            const bool some_nan = __any_sync(0xffffffffu, nan);
-            if (some_nan) {
-                top = 0u;
+            if (__any_sync(0xffffffffu, nan)) {
 #pragma unroll
-                for (int j = 0; j < 2; ++j) top = max(top, vb[j] == 255u ? 0u : vb[j]);
-            }
-            top = __reduce_max_sync(0xffffffffu, top);
-            if (top > vtop) {                                  // rarely: the scales of a head's values are much alike
-                const float f = relative_scale(vtop, top);
-#pragma unroll
-                for (int n = 0; n < HT; ++n)
-#pragma unroll
-                    for (int k = 0; k < C::MT; ++k)
-#pragma unroll
-                        for (int x = 0; x < 4; ++x) o[n][k][x] *= f;
-                vtop = top;
-            }
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                vs[j] = relative_scale(vb[j], vtop);
-                if (some_nan) {
+                for (int j = 0; j < 2; ++j) {
                     if (kb[j] == 255u) ks[j] = __uint_as_float(0x7fc00000u);
-                    if (vb[j] == 255u) vs[j] = __uint_as_float(0x7fc00000u);
+                    if (vb[j] == 255u) vlog[j] = __uint_as_float(0x7fc00000u);
                 }
             }
         }
@@ -336,6 +323,46 @@ __global__ void __launch_bounds__(kWarps * 32, CTAS) step_mma_kernel(const StepA
                     for (int k = 0; k < C::MT; ++k) { o[n][k][x] *= f; o[n][k][2 + x] *= f; }
                 }
             }
+            float w[2][2];                                     // 8 bits: log2 of the operands
+            if constexpr (F8) {
+                const auto operands = [&] {
+                    bool over = false;
+#pragma unroll
+                    for (int j = 0; j < 2; ++j)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            w[j][e] = fmaf(sc[n][2 * j + e], fs[n][e], vlog[j] - wbase[n][e]);
+                            over |= w[j][e] > kTop;
+                        }
+                    return __any_sync(0xffffffffu, over);
+                };
+                if (operands()) {
+                    // a value row of zeros has a scale of 1 but no weight in the sum: left out
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        uint32_t any = 0u;
+#pragma unroll
+                        for (int b = 0; b < D; b += 64) {
+                            uint32_t u[4] = {0u, 0u, 0u, 0u};
+                            if (b + 16 * t < D) load_shared(st0 + C::at(g, D + b + 16 * t) + 8 * j * C::ROW, u);
+                            any |= (u[0] | u[1] | u[2] | u[3]) & 0x7f7f7f7fu;
+                        }
+                        any |= __shfl_xor_sync(0xffffffffu, any, 1); any |= __shfl_xor_sync(0xffffffffu, any, 2);
+                        if (any == 0u) vlog[j] -= INFINITY;
+                    }
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        float top = fmaxf(fmaf(sc[n][e], fs[n][e], vlog[0]), fmaf(sc[n][2 + e], fs[n][e], vlog[1]));
+#pragma unroll
+                        for (int b = 4; b < 32; b <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, b));
+                        const float moved = fmaxf(wbase[n][e], rintf(top) - kLevel), f = exp2_fast(wbase[n][e] - moved);
+                        wbase[n][e] = moved;
+#pragma unroll
+                        for (int k = 0; k < C::MT; ++k) { o[n][k][e] *= f; o[n][k][2 + e] *= f; }
+                    }
+                    operands();
+                }
+            }
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
                 float x[2];
@@ -343,16 +370,21 @@ __global__ void __launch_bounds__(kWarps * 32, CTAS) step_mma_kernel(const StepA
                 for (int e = 0; e < 2; ++e) {
                     x[e] = exp2_fast(fmaf(sc[n][2 * j + e], fs[n][e], -base[n][e]));
                     l[n][e] += x[e];
-                    if constexpr (F8) x[e] *= vs[j];
+                    if constexpr (F8) x[e] = exp2_fast(w[j][e]);
                 }
-                if constexpr (F8) pb[n][j] = transposed(pack_f16x2(x[0], x[1]));      // relative 2^-11 on terms that add up
-                else {
-                    // two operands in bf16, the number and what its rounding left: together off by 2^-16 of it.  One alone (2^-8) is seen in the result: 0.0023
-                    // from 64 bits (2-norms, 64 sequences up to 4096, 8 x 4 heads of 128), where the result's own rounding to bf16 is 0.0017.
-                    const uint32_t hi = pack_bf16x2(x[0], x[1]);
-                    pb[n][j] = transposed(hi);
-                    pl[n][j] = transposed(pack_bf16x2(x[0] - __uint_as_float(hi << 16), x[1] - __uint_as_float(hi & 0xffff0000u)));
+                // Two operands of 16 bits, the number and what its rounding left: together off by 2^-16 of it (bf16) or 2^-22 (f16, see kTop).  One alone (2^-8 or
+                // 2^-11) is seen in the result: in bf16 0.0023 from 64 bits (2-norms, 64 sequences up to 4096, 8 x 4 heads of 128), where the result's own
+                // rounding to bf16 is 0.0017.
+                uint32_t hi, lo;
+                if constexpr (F8) {
+                    hi = pack_f16x2(x[0], x[1]);
+                    const float2 held = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+                    lo = pack_f16x2(x[0] - held.x, x[1] - held.y);
+                } else {
+                    hi = pack_bf16x2(x[0], x[1]);
+                    lo = pack_bf16x2(x[0] - __uint_as_float(hi << 16), x[1] - __uint_as_float(hi & 0xffff0000u));
                 }
+                pb[n][j] = transposed(hi); pl[n][j] = transposed(lo);
             }
         }
         // ---- O^T += V^T P^T: rows g and g + 8 of m-tile (k VE + e) / 2 are d = 8 VE k + VE g + e and the next
@@ -371,7 +403,10 @@ __global__ void __launch_bounds__(kWarps * 32, CTAS) step_mma_kernel(const StepA
                         e4m3x4_half2(__byte_perm(w[0][x], w[1][x], y ? 0x7362 : 0x5140), va[0], va[1]);
                         e4m3x4_half2(__byte_perm(w[2][x], w[3][x], y ? 0x7362 : 0x5140), va[2], va[3]);
 #pragma unroll
-                        for (int n = 0; n < HT; ++n) mma<true>(o[n][(k * C::VE + 4 * x) / 2 + y], va, pb[n][0], pb[n][1]);
+                        for (int n = 0; n < HT; ++n) {
+                            mma<true>(o[n][(k * C::VE + 4 * x) / 2 + y], va, pb[n][0], pb[n][1]);
+                            mma<true>(o[n][(k * C::VE + 4 * x) / 2 + y], va, pl[n][0], pl[n][1]);
+                        }
                     }
                 } else {
                     const uint32_t va[4] = {__byte_perm(w[0][x], w[1][x], 0x5410), __byte_perm(w[0][x], w[1][x], 0x7632),
@@ -390,7 +425,6 @@ __global__ void __launch_bounds__(kWarps * 32, CTAS) step_mma_kernel(const StepA
     const bool any_bad = __syncthreads_or(bad);
     float* const sml = reinterpret_cast<float*>(smem);         // [warps][heads][2]
     float* const so = sml + kWarps * C::HEADS * 2;             // [warps][heads][D]
-    const float unit = F8 ? scale_value(vtop) : 1.f;
 #pragma unroll
     for (int n = 0; n < HT; ++n)
 #pragma unroll
@@ -398,11 +432,13 @@ __global__ void __launch_bounds__(kWarps * 32, CTAS) step_mma_kernel(const StepA
             const int at = warp * C::HEADS + 8 * n + 2 * t + x;
 #pragma unroll
             for (int b = 4; b < 32; b <<= 1) l[n][x] += __shfl_xor_sync(0xffffffffu, l[n][x], b);
+            const float top = m[n][x] == -INFINITY ? 0.f : base[n][x];
+            const float unit = F8 ? exp2f(0.5f * (wbase[n][x] - top)) : 1.f;         // twice, for 2^(w - base) alone may be out of range
             if (g == 0) { sml[at * 2] = m[n][x] == -INFINITY ? -INFINITY : base[n][x]; sml[at * 2 + 1] = l[n][x]; }
 #pragma unroll
             for (int k = 0; k < C::VP; ++k)
 #pragma unroll
-                for (int e = 0; e < C::VE; ++e) so[at * D + 8 * C::VE * k + C::VE * g + e] = o[n][(k * C::VE + e) / 2][2 * (e & 1) + x] * unit;
+                for (int e = 0; e < C::VE; ++e) so[at * D + 8 * C::VE * k + C::VE * g + e] = o[n][(k * C::VE + e) / 2][2 * (e & 1) + x] * unit * unit;
         }
     __syncthreads();
     for (int z = threadIdx.x; z < heads * DR; z += kWarps * 32) {

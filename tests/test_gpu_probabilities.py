@@ -6,7 +6,7 @@ import pytest
 import torch
 
 import dwarf_b200
-from tests.serving_util import HALF, attention64
+from tests.serving_util import HALF, attention64, quantize64
 from tests.test_gpu_paged import held_as, make_cache
 
 pytestmark = pytest.mark.gpu
@@ -36,3 +36,94 @@ def test_bf16_pages(H, G, D, page):
             o, spread, ds = attention64(qs, r[:, 0], r[:, 1], sc)
             off, bound = (out[s, h * G:(h + 1) * G] - o).abs(), paged_bound(qs, r, sc, o, spread, ds, 2.0 ** -16)
             assert (off <= bound).all(), (lengths[s], h, (off / bound).max())
+
+
+def cache8(rows, page):
+    """Pages in 8 bits that hold rows [n,H,2,D] of every sequence: (kv, scale, table, the values they stand for)."""
+    S, per = len(rows), [-(-r.shape[0] // page) for r in rows]
+    _, H, _, D = rows[0].shape
+    x = torch.zeros(sum(per), H, page, 2, D)
+    table, at = torch.full((S, max(per)), -1, dtype=torch.int32), 0
+    for s, r in enumerate(rows):
+        for c in range(per[s]):
+            part = r[c * page:(c + 1) * page]
+            x[at, :, :part.shape[0]] = part.transpose(0, 1)
+            table[s, c] = at
+            at += 1
+    v, sc = quantize64(x)
+    byte = (torch.log2(sc) + 127).to(torch.uint8)
+    return v.float().to(E4).to(DEV), byte.view(torch.float8_e8m0fnu).to(DEV), table.to(DEV), [held_as(r, E4) for r in rows]
+
+
+def e4m3_bound(qs, r, sc, o, spread, ds, p):
+    """As paged_bound: f16 keeps 2^-11 of a number and 2^-11 of what is left of it; exponents up to 64 are rounded three times (2^-18 each, times ln 2); below its
+    normal range f16 is off by 2^-25, where the largest term of the result is at 2^9.5 (and values of a row are within 2 of its largest); queries are off by 2^-24 of
+    their largest element, at keys that carry weight."""
+    far = r.shape[0] * 2.0 ** -33.5 * (p * r[:, 1].abs().max(1).values).max(1).values[:, None]
+    live = p.max(0).values > 1e-12
+    dq = 2 * sc * 2.0 ** -24 * qs.abs().max() * r[live, 0].abs().sum(1).max()
+    return paged_bound(qs, r, sc, o, spread, ds, 2.0 ** -22 + 3 * 2.0 ** -18 + dq) + 1.01 * far
+
+
+def check8(rows, q, page, sc):
+    S, H = len(rows), rows[0].shape[1]
+    G = q.shape[1] // H
+    kv, ks, table, held = cache8(rows, page)
+    n = torch.tensor([r.shape[0] for r in rows], dtype=torch.int32, device=DEV)
+    out = dwarf_b200.paged_attention_step(q.to(DEV), None, None, kv, table, n, kv_scale=ks, scale=sc).double().cpu()
+    for s in range(S):
+        for h in range(H):
+            qs, r = q[s, h * G:(h + 1) * G].double(), held[s][:, h]
+            o, spread, ds = attention64(qs, r[:, 0], r[:, 1], sc)
+            off, bound = (out[s, h * G:(h + 1) * G] - o).abs(), e4m3_bound(qs, r, sc, o, spread, ds, torch.softmax(sc * qs @ r[:, 0].T, 1))
+            assert (off <= bound).all(), (s, h, (off / bound).max())
+
+
+SHAPES = [(2, 1, 32, 16), (1, 4, 128, 64), (2, 3, 96, 48), (1, 12, 64, 32), (1, 17, 128, 16), (2, 8, 80, 32), (1, 2, 48, 16), (1, 9, 32, 10)]
+
+
+@pytest.mark.parametrize("H,G,D,page", SHAPES)
+def test_e4m3_pages(H, G, D, page):
+    g = torch.Generator().manual_seed(D + G)
+    rows = [torch.randn(n, H, 2, D, generator=g) * torch.exp(0.7 * torch.randn(n, H, 2, 1, generator=g)) for n in (1, 2, 20, 45, 300)]
+    check8(rows, torch.randn(len(rows), H * G, D, generator=g).to(BF), page, 0.02)
+
+
+@pytest.mark.parametrize("H,G,D,page", SHAPES)
+@pytest.mark.parametrize("above", [12, 20, 26, 60])
+def test_e4m3_value_rows_that_carry_no_weight_take_no_bits(H, G, D, page, above):
+    """One value row 2^above the others, first, in the middle and last, whose key's score is 100 or more below: e^-100 2^60 of it is below 2^-84."""
+    g = torch.Generator().manual_seed(D + G + above)
+    n, sc = 150, 1 / math.sqrt(D)
+    far = [0, 75, 149]
+    q0 = torch.randn(1, H, 1, D, generator=g)
+    q = (q0 + 0.05 * torch.randn(len(far), H, G, D, generator=g)).reshape(len(far), H * G, D).to(BF)
+    rows = [0.3 * torch.randn(n, H, 2, D, generator=g) for _ in far]
+    for r, at in zip(rows, far):
+        r[at, :, 0] = -120 / sc * q0[0, :, 0] / q0[0, :, 0].square().sum(-1, keepdim=True)
+        r[at, :, 1] = 2.0 ** above
+    check8(rows, q, page, sc)
+
+
+@pytest.mark.parametrize("H,G,D,page", SHAPES)
+def test_e4m3_value_rows_of_zeros_take_no_bits(H, G, D, page):
+    """A row of zeros is held with a scale of 1, which says nothing of its size: values of 2^-30 beside it, first, last and in a tile of its own."""
+    g = torch.Generator().manual_seed(D + G)
+    rows = [torch.randn(150, H, 2, D, generator=g) * torch.tensor([1.0, 2.0 ** -30])[None, None, :, None] for _ in range(3)]
+    rows[0][0, :, 1], rows[1][149, :, 1], rows[2][16:40, :, 1] = 0, 0, 0
+    rows[2][16:40, :, 1, 0] = -0.0
+    check8(rows, torch.randn(3, H * G, D, generator=g).to(BF), page, 0.02)
+
+
+def test_e4m3_growing_values_and_scores():
+    """Scores and scales that grow along the sequence: bases move at every tile."""
+    g = torch.Generator().manual_seed(5)
+    H, G, D, n = 2, 4, 64, 260
+    q0 = torch.randn(1, H, 1, D, generator=g)
+    q = (q0 + 0.02 * torch.randn(2, H, G, D, generator=g)).reshape(2, H * G, D).to(BF)
+    rows = [torch.randn(n, H, 2, D, generator=g) for _ in range(2)]
+    step = torch.arange(n)[:, None, None] / n
+    for r, sign in zip(rows, (1, -1)):
+        r[:, :, 0] = sign * 40 * step * math.sqrt(D) * q0[0, :, 0] / q0[0, :, 0].square().sum(-1, keepdim=True)
+        r[:, :, 1] *= torch.exp2(60 * step)
+    check8(rows, q, 32, 1 / math.sqrt(D))
