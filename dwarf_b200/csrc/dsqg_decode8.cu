@@ -211,14 +211,17 @@ decode8_kernel(const DecodeArgs a, uint8_t* __restrict__ scale, const Taps t) {
 //
 // Taps are the 16 rows of mma.sync (m16n8k16, f16 in, fp32 sums), the query stands in all eight columns: scores = K q without a shuffle, and after the softmax
 // O^T += V^T p without one, p turned from a result into an operand by movmatrix.  e4m3 becomes f16 exactly; the query becomes f16 after a power of two
-// that brings its largest element to [1, 2); the keys' scales multiply the scores, the values' scales the probabilities, relative to the largest scale
-// of the step.  What bounds the step is instructions, not memory: some 1180 a warp instead of the 1730 of the form above, whose rows go to fp32 one by one.
+// that brings its largest element to [1, 2); the keys' scales multiply the scores.  An operand of the second product is 2^(score + exponent of the value row's
+// scale - w), w such that the largest is at 2^12: what is largest in the result is largest in f16, whatever scales other rows have.  It stands as two f16 numbers,
+// itself in the even columns and what its rounding left in the odd ones, off by 2^-22 together.  What bounds the step is instructions, not memory: some 1180 a warp instead of the 1730 of the form above, whose rows go to fp32 one by one.
 // A lane asks for the pieces of key rows g and g + 8 that it needs itself (lane (g, t): piece t); value rows go to shared memory as rows, even ones in
 // front of odd ones and pieces exchanged so that rows 2 t, 2 t + 1, 2 t + 8, 2 t + 9 are read without bank conflicts.
 template <int D> struct Mma {
     static constexpr int KB = D >= 64 ? 16 : 8, KP = D / (4 * KB);           // bytes of a piece of a row, pieces a lane
     static constexpr int VB = D / 8;                                         // bytes of a value row for a lane
     static constexpr int TILES = 3, W = D == 128 ? 2 : 4;                    // 16-tap tiles a pass; warps a block
+    // Blocks an SM: us at 256 x 12 x 64 with five, six, seven 8.3, 7.9, 9.2 (spills); at 256 x 8 x 32 5.7, 6.0, 5.0, a launch's blocks then fit beside the last one's
+    static constexpr int CTAS = D == 32 ? 7 : 6;
     static constexpr int KTILE = 16 * D, STAGE = TILES * 2 * KTILE;          // key rows, then value rows
     __device__ static __forceinline__ int value_at(int row, int byte) {
         const int r = (row & 8) | (row & 1) << 2 | (row >> 1 & 3);
@@ -237,7 +240,7 @@ template <int WORDS> __device__ __forceinline__ void words_of(const void* p, uin
 }
 
 template <int D, bool PDL>
-__global__ void __launch_bounds__(Mma<D>::W * 32, 6) decode8_mma_kernel(const DecodeArgs a, uint8_t* __restrict__ scale, const Taps t) {
+__global__ void __launch_bounds__(Mma<D>::W * 32, Mma<D>::CTAS) decode8_mma_kernel(const DecodeArgs a, uint8_t* __restrict__ scale, const Taps t) {
     using C = Mma<D>;
     constexpr int TILES = C::TILES, KP = C::KP, KB = C::KB, VEC = D / 4, STEPS = D / 16, E = KB / 4;
     if constexpr (!PDL) stream_wait();
@@ -253,14 +256,13 @@ __global__ void __launch_bounds__(Mma<D>::W * 32, 6) decode8_mma_kernel(const De
     char* const values = smem[warp] + TILES * C::KTILE;
 
     uint32_t qb[STEPS][2];
-    float fs = 0.f, m = -INFINITY, l = 0.f, o[STEPS][4];
+    float fs = 0.f, m = -INFINITY, l = 0.f, wbase = -1e30f, o[STEPS][4];
 #pragma unroll
     for (int k = 0; k < STEPS; ++k) {
         qb[k][0] = qb[k][1] = 0u;
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[k][e] = 0.f;
     }
-    uint32_t vtop = 0u;
 #pragma unroll 1
     for (int j0 = 0; j0 < t.J; j0 += 16 * TILES) {             // one pass for the usual tap counts
         uint32_t sb[TILES][2];
@@ -343,8 +345,8 @@ __global__ void __launch_bounds__(Mma<D>::W * 32, 6) decode8_mma_kernel(const De
         } else asm volatile("cp.async.wait_all;" ::: "memory");
         __syncwarp();
         // ---- scores: taps g and g + 8 of a tile, the same in every column
-        float sc[TILES][2], mx = m;
-        uint32_t top = vtop;
+        float sc[TILES][2], vlog[TILES][2], mx = m, top = -INFINITY;
+        bool one = false;
 #pragma unroll
         for (int i = 0; i < TILES; ++i) {
             float c[4] = {0.f, 0.f, 0.f, 0.f};
@@ -366,33 +368,56 @@ __global__ void __launch_bounds__(Mma<D>::W * 32, 6) decode8_mma_kernel(const De
                 sc[i][x] = tap[i][x] ? fmaf(c[2 * x] * row_scale(sb[i][x] & 255u), fs, bias) : -INFINITY;
                 mx = fmaxf(mx, sc[i][x]);
                 const uint32_t vb = sb[i][x] >> 8;
-                if (tap[i][x] && vb != 255u) top = max(top, vb);
+                vlog[i][x] = vb == 255u ? __uint_as_float(0x7fc00000u) : log2_scale(vb);
+                one |= tap[i][x] && vb == 127u;
             }
         }
-        top = __reduce_max_sync(0xffffffffu, top);
+        if (__any_sync(0xffffffffu, one)) {                    // a value row of zeros has a scale of 1 but no weight in the sum: left out
 #pragma unroll
-        for (int b = 4; b < 32; b <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, b));
+            for (int i = 0; i < TILES; ++i)
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                    uint32_t any = 0u;
+#pragma unroll
+                    for (int k = 0; k < KP; ++k) {
+                        uint32_t u[E];
+                        words_of(values + i * C::KTILE + C::value_at(g + 8 * x, (4 * k + tig) * KB), u);
+#pragma unroll
+                        for (int e = 0; e < E; ++e) any |= u[e] & 0x7f7f7f7fu;
+                    }
+                    any |= __shfl_xor_sync(0xffffffffu, any, 1); any |= __shfl_xor_sync(0xffffffffu, any, 2);
+                    if (any == 0u) vlog[i][x] -= INFINITY;
+                }
+        }
+#pragma unroll
+        for (int i = 0; i < TILES; ++i)
+#pragma unroll
+            for (int x = 0; x < 2; ++x) top = fmaxf(top, sc[i][x] + vlog[i][x]);
+#pragma unroll
+        for (int b = 4; b < 32; b <<= 1) {
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, b));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, b));
+        }
+        const float moved = fmaxf(wbase, rintf(top) - 12.f);
         const float base = mx == -INFINITY ? 0.f : mx;
-        if (j0) {                                              // a later pass: what was summed so far is against the old maximum and the old scale
-            const float f = exp2f(m - base), fv = f * __uint_as_float((uint32_t)max(127 + (int)vtop - (int)top, 0) << 23);
-            l *= f;
+        if (j0) {                                              // a later pass: what was summed so far is against the old maximum and the old w
+            const float fv = exp2f(wbase - moved);
+            l *= exp2f(m - base);
 #pragma unroll
             for (int k = 0; k < STEPS; ++k)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) o[k][e] *= fv;
         }
-        m = mx; vtop = top;
+        m = mx; wbase = moved;
 #pragma unroll
         for (int i = 0; i < TILES; ++i) {
             uint32_t pb[2];
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
-                const float p = exp2f(sc[i][x] - base);
-                l += p;
-                const uint32_t vb = sb[i][x] >> 8;
-                const float w = !tap[i][x] ? 0.f : p * (vb == 255u ? __uint_as_float(0x7fc00000u) : __uint_as_float((uint32_t)max(127 + (int)vb - (int)top, 0) << 23));
-                // to f16, as the operand of the product: relative 2^-11 on terms that add up
-                asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(pb[x]) : "r"(f16x2(w, w)));
+                l += exp2_fast(sc[i][x] - base);
+                const float w = tap[i][x] ? exp2_fast(sc[i][x] + (vlog[i][x] - wbase)) : 0.f;
+                const __half hi = __float2half_rn(w);
+                asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(pb[x]) : "r"(f16x2(w, w - __half2float(hi))));
             }
             uint32_t w[4][C::VB / 4];
 #pragma unroll
@@ -412,10 +437,11 @@ __global__ void __launch_bounds__(Mma<D>::W * 32, 6) decode8_mma_kernel(const De
 #pragma unroll
     for (int b = 4; b < 32; b <<= 1) l += __shfl_xor_sync(0xffffffffu, l, b);
     if (tig == 0) {                                            // d = VB g + 2 (m-tile), + 1
-        const float inv = l == 0.f ? 0.f : (a.head_gain ? a.head_gain[h] : 1.f) / l * scale_value(vtop);
+        const float inv = l == 0.f ? 0.f : (a.head_gain ? a.head_gain[h] : 1.f) / l;
+        const float unit = exp2f(0.5f * (wbase - (m == -INFINITY ? 0.f : m)));         // twice, for 2^(w - m) alone may be out of range
         uint32_t y[STEPS];
 #pragma unroll
-        for (int k = 0; k < STEPS; ++k) y[k] = pack_bf16x2(o[k][0] * inv, o[k][2] * inv);
+        for (int k = 0; k < STEPS; ++k) y[k] = pack_bf16x2((o[k][0] + o[k][1]) * unit * unit * inv, (o[k][2] + o[k][3]) * unit * unit * inv);
         uint32_t* const to = reinterpret_cast<uint32_t*>(static_cast<__nv_bfloat16*>(a.out) + (size_t)sh * D + g * C::VB);
 #pragma unroll
         for (int k = 0; k < STEPS; k += 2) *reinterpret_cast<uint2*>(to + k) = make_uint2(y[k], y[k + 1]);

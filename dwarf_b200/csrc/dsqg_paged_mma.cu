@@ -53,8 +53,6 @@ template <int WORDS> __device__ __forceinline__ void load_shared(uint32_t from, 
     else if constexpr (WORDS == 2) asm volatile("ld.shared.v2.b32 {%0,%1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(from) : "memory");
     else asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w[0]) : "r"(from) : "memory");
 }
-// 2^x (2 ulp; results below 2^-126 become 0)
-__device__ __forceinline__ float exp2_fast(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
 __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
     const __half2 h = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&h);
@@ -66,8 +64,6 @@ __device__ __forceinline__ uint32_t transposed(uint32_t x) {
     asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
     return y;
 }
-// log2 of the scale that a byte stands for
-__device__ __forceinline__ float log2_scale(uint32_t byte) { return __uint_as_float(0x4b000000u | byte) - 8388735.f; }
 
 // DR: columns of the cache; D: of the products, DR rounded up to 32.  What is behind the DR columns of a key or value row is zero in shared memory, from the start on.
 template <int DR, bool F8, int HT, int STAGES>

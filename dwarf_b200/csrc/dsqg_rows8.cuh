@@ -27,6 +27,8 @@ __device__ __forceinline__ uint32_t row_scale_byte(uint32_t top) {
 __device__ __forceinline__ float scale_value(uint32_t byte) {
     return byte == 255u ? __uint_as_float(0x7fc00000u) : __uint_as_float(byte ? byte << 23 : 0x00400000u);
 }
+// log2 of the scale that a byte below 255 stands for (of 0: -127)
+__device__ __forceinline__ float log2_scale(uint32_t byte) { return __uint_as_float(0x4b000000u | byte) - 8388735.f; }
 // 1 / scale of a byte that row_scale_byte gave (1 .. 247, or 255: NaN)
 __device__ __forceinline__ float scale_inverse(uint32_t byte) { return byte == 255u ? __uint_as_float(0x7fc00000u) : __uint_as_float((254u - byte) << 23); }
 
@@ -48,6 +50,9 @@ __device__ __forceinline__ void e4m3x4_float(uint32_t w, float* x) {
     const float2 a = __half22float2(e4m3x2_half2(w & 0xffffu)), b = __half22float2(e4m3x2_half2(w >> 16));
     x[0] = a.x; x[1] = a.y; x[2] = b.x; x[3] = b.y;
 }
+
+// 2^x (2 ulp; results below 2^-126 become 0)
+__device__ __forceinline__ float exp2_fast(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
 
 template <int WIDTH> __device__ __forceinline__ uint32_t group_max(uint32_t x) {
 #pragma unroll

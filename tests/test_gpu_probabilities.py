@@ -127,3 +127,65 @@ def test_e4m3_growing_values_and_scores():
         r[:, :, 0] = sign * 40 * step * math.sqrt(D) * q0[0, :, 0] / q0[0, :, 0].square().sum(-1, keepdim=True)
         r[:, :, 1] *= torch.exp2(60 * step)
     check8(rows, q, 32, 1 / math.sqrt(D))
+
+
+# ---- rings
+MANY, FEW = tuple(range(100)) + (128,), (0, 1, 2, 3, 4, 5, 6, 8, 16, 32, 40)
+
+
+def check_ring8(rows, q, offsets):
+    """rows [S,H,R,2,D]: what the rings hold; the new token of a sequence is what stands at slot 0."""
+    S, H, R, _, D = rows.shape
+    v, sc = quantize64(rows)
+    kv, ks = v.float().to(E4).to(DEV), (torch.log2(sc) + 127).to(torch.uint8).view(torch.float8_e8m0fnu).to(DEV)
+    held, head, sc = held_as(rows, E4), torch.zeros(S, dtype=torch.int32, device=DEV), 1 / math.sqrt(D)
+    new = rows[:, :, 0].to(BF)
+    assert torch.equal(held_as(new, E4), held[:, :, 0])               # the new token's rows in bf16 are held as those in fp32
+    pb = torch.zeros(len(offsets), H, device=DEV)
+    for overlap in (False, True):
+        out = dwarf_b200.dsqg_decode_step_kv(q.to(DEV), *(new[:, :, i].contiguous().to(DEV) for i in (0, 1)), kv, head, pb, None, None, offsets, None, overlap=overlap,
+                                             kv_scale=ks).double().cpu()
+        at = [(0 - o) % R for o in offsets]
+        for s in range(S):
+            for h in range(H):
+                qs, r = q[s, h][None].double(), held[s, h, at]
+                o, spread, ds = attention64(qs, r[:, 0], r[:, 1], sc)
+                off, bound = (out[s, h] - o[0]).abs(), e4m3_bound(qs, r, sc, o, spread, ds, torch.softmax(sc * qs @ r[:, 0].T, 1))[0]
+                assert (off <= bound).all(), (s, h, (off / bound).max())
+
+
+def ring_rows(S, H, D, offsets, g):
+    return torch.randn(S, H, max(offsets) + 1, 2, D, generator=g).to(BF).float()
+
+
+@pytest.mark.parametrize("H,D", [(2, 32), (3, 64), (1, 128)])
+@pytest.mark.parametrize("offsets", [FEW, MANY], ids=["one_pass", "passes"])
+def test_ring8(H, D, offsets):
+    g = torch.Generator().manual_seed(D)
+    rows, q = ring_rows(3, H, D, offsets, g), torch.randn(3, H, D, generator=g).to(BF)
+    check_ring8(rows, 0.05 * q, offsets)
+
+
+@pytest.mark.parametrize("H,D", [(2, 32), (3, 64), (1, 128), (2, 48)])
+@pytest.mark.parametrize("offsets", [FEW, MANY], ids=["one_pass", "passes"])
+@pytest.mark.parametrize("above", [12, 20, 26, 60])
+def test_ring8_value_rows_that_carry_no_weight_take_no_bits(H, D, offsets, above):
+    g = torch.Generator().manual_seed(D + above)
+    S = 3
+    rows, q0 = 0.25 * ring_rows(S, H, D, offsets, g), torch.randn(S, H, D, generator=g)
+    R = rows.shape[2]
+    for s, o in enumerate((0, offsets[5], offsets[-1])):
+        rows[s, :, (0 - o) % R, 0] = (-120 * math.sqrt(D) * q0[s] / q0[s].square().sum(-1, keepdim=True)).to(BF).float()
+        rows[s, :, (0 - o) % R, 1] = 2.0 ** above
+    check_ring8(rows, q0.to(BF), offsets)
+
+
+@pytest.mark.parametrize("H,D", [(2, 32), (3, 64), (1, 128)])
+@pytest.mark.parametrize("offsets", [FEW, MANY], ids=["one_pass", "passes"])
+def test_ring8_value_rows_of_zeros_take_no_bits(H, D, offsets):
+    g = torch.Generator().manual_seed(D)
+    rows = ring_rows(3, H, D, offsets, g) * torch.tensor([1.0, 2.0 ** -30])[:, None]
+    R = rows.shape[2]
+    for s, o in enumerate((0, offsets[5], offsets[-1])):
+        rows[s, :, (0 - o) % R, 1] = -0.0
+    check_ring8(rows, 0.05 * torch.randn(3, H, D, generator=g).to(BF), offsets)
