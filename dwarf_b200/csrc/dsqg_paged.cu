@@ -217,7 +217,7 @@ __global__ void __launch_bounds__(kStepThreads) step_kernel(const StepArgs a) {
     Row next = fetch(r.first + group);
     for (int p0 = r.first; p0 < r.end; p0 += STEP) {
         const Row now = next;
-        next = fetch(p0 + STEP + group);                       // on its way while this one is used
+        next = fetch(p0 + STEP + group);                       // on its way while this one is used; at most 2^31 - 257 + 255
         const float (&k)[8] = now.k, (&v)[8] = now.v;
         const bool valid = now.valid;
 #pragma unroll
@@ -283,7 +283,7 @@ template <int W> __global__ void __launch_bounds__(kJoinWarps * 32) join_kernel(
     int n = 0;
     if (row < rows) {
         const Range r = range_of(a, row / (a.c.H * a.G), 0);
-        n = r.length ? (r.length + a.chunk - 1) / a.chunk : 1;
+        n = r.length ? (r.length - 1) / a.chunk + 1 : 1;
     }
     stream_wait();
     const float2* ml = a.ml + (long long)row * a.parts;

@@ -39,7 +39,7 @@ __device__ __forceinline__ Range range_of(const StepArgs& a, int s, int part) {
     r.bad = r.length < 0 || r.length > a.limit;
     if (r.bad) r.length = 0;
     r.first = part * a.chunk;
-    r.end = min(r.length, r.first + a.chunk);
+    r.end = r.first + min(r.length - r.first, a.chunk);        // up to 2^31 - 256 positions: first + chunk may be beyond an int
     return r;
 }
 
