@@ -315,8 +315,10 @@ __global__ void __launch_bounds__(kWarps * 32, CTAS) step_mma_kernel(const StepA
                     lim[n][x] = mn + kSlack / fs[n][x];
                     base[n][x] = mn == -INFINITY ? 0.f : mn * fs[n][x];
                     l[n][x] *= f;
+                    if constexpr (!F8) {                           // in 8 bits the sums of values have a base of their own
 #pragma unroll
-                    for (int k = 0; k < C::MT; ++k) { o[n][k][x] *= f; o[n][k][2 + x] *= f; }
+                        for (int k = 0; k < C::MT; ++k) { o[n][k][x] *= f; o[n][k][2 + x] *= f; }
+                    }
                 }
             }
             float w[2][2];                                     // 8 bits: log2 of the operands

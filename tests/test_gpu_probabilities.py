@@ -21,13 +21,15 @@ def paged_bound(qs, r, sc, o, spread, ds, p_half):
 
 
 @pytest.mark.parametrize("H,G,D,page", [(2, 1, 32, 16), (1, 4, 128, 64), (2, 3, 96, 48), (1, 12, 64, 32), (1, 17, 128, 16), (2, 8, 80, 32), (1, 2, 48, 16)])
-def test_bf16_pages(H, G, D, page):
+@pytest.mark.parametrize("room", [0, 1 << 20], ids=["short_parts", "one_part"])
+def test_bf16_pages(H, G, D, page, room):
     """bf16 keeps 2^-8 of a number and 2^-8 of what is left of it: 2^-16.  Scores near one another, so that their own error is far below, and values that
     cancel, so that the result's rounding is too."""
     g = torch.Generator().manual_seed(D + G)
     lengths, sc = [1, 2, 20, 45, 300, 1000], 0.02
     S = len(lengths)
     kv, _, table, rows = make_cache(lengths, H, page, D, BF, g)
+    table = torch.nn.functional.pad(table, (0, max(0, room // page - table.shape[1])), value=-1)
     q = torch.randn(S, H * G, D, generator=g).to(BF)
     out = dwarf_b200.paged_attention_step(q.to(DEV), None, None, kv, table, torch.tensor(lengths, dtype=torch.int32, device=DEV), scale=sc).double().cpu()
     for s in range(S):
@@ -65,10 +67,12 @@ def e4m3_bound(qs, r, sc, o, spread, ds, p):
     return paged_bound(qs, r, sc, o, spread, ds, 2.0 ** -22 + 3 * 2.0 ** -18 + dq) + 1.01 * far
 
 
-def check8(rows, q, page, sc):
+def check8(rows, q, page, sc, room=0):
+    """room: positions that the table has columns for, which decide how long a part is."""
     S, H = len(rows), rows[0].shape[1]
     G = q.shape[1] // H
     kv, ks, table, held = cache8(rows, page)
+    table = torch.nn.functional.pad(table, (0, max(0, room // page - table.shape[1])), value=-1)
     n = torch.tensor([r.shape[0] for r in rows], dtype=torch.int32, device=DEV)
     out = dwarf_b200.paged_attention_step(q.to(DEV), None, None, kv, table, n, kv_scale=ks, scale=sc).double().cpu()
     for s in range(S):
@@ -83,15 +87,17 @@ SHAPES = [(2, 1, 32, 16), (1, 4, 128, 64), (2, 3, 96, 48), (1, 12, 64, 32), (1, 
 
 
 @pytest.mark.parametrize("H,G,D,page", SHAPES)
-def test_e4m3_pages(H, G, D, page):
+@pytest.mark.parametrize("room", [0, 1 << 20], ids=["short_parts", "one_part"])
+def test_e4m3_pages(H, G, D, page, room):
     g = torch.Generator().manual_seed(D + G)
     rows = [torch.randn(n, H, 2, D, generator=g) * torch.exp(0.7 * torch.randn(n, H, 2, 1, generator=g)) for n in (1, 2, 20, 45, 300)]
-    check8(rows, torch.randn(len(rows), H * G, D, generator=g).to(BF), page, 0.02)
+    check8(rows, torch.randn(len(rows), H * G, D, generator=g).to(BF), page, 0.02, room)
 
 
 @pytest.mark.parametrize("H,G,D,page", SHAPES)
+@pytest.mark.parametrize("room", [0, 1 << 20], ids=["short_parts", "one_part"])
 @pytest.mark.parametrize("above", [12, 20, 26, 60])
-def test_e4m3_value_rows_that_carry_no_weight_take_no_bits(H, G, D, page, above):
+def test_e4m3_value_rows_that_carry_no_weight_take_no_bits(H, G, D, page, above, room):
     """One value row 2^above the others, first, in the middle and last, whose key's score is 100 or more below: e^-100 2^60 of it is below 2^-84."""
     g = torch.Generator().manual_seed(D + G + above)
     n, sc = 150, 1 / math.sqrt(D)
@@ -102,31 +108,34 @@ def test_e4m3_value_rows_that_carry_no_weight_take_no_bits(H, G, D, page, above)
     for r, at in zip(rows, far):
         r[at, :, 0] = -120 / sc * q0[0, :, 0] / q0[0, :, 0].square().sum(-1, keepdim=True)
         r[at, :, 1] = 2.0 ** above
-    check8(rows, q, page, sc)
+    check8(rows, q, page, sc, room)
 
 
 @pytest.mark.parametrize("H,G,D,page", SHAPES)
-def test_e4m3_value_rows_of_zeros_take_no_bits(H, G, D, page):
+@pytest.mark.parametrize("room", [0, 1 << 20], ids=["short_parts", "one_part"])
+def test_e4m3_value_rows_of_zeros_take_no_bits(H, G, D, page, room):
     """A row of zeros is held with a scale of 1, which says nothing of its size: values of 2^-30 beside it, first, last and in a tile of its own."""
     g = torch.Generator().manual_seed(D + G)
     rows = [torch.randn(150, H, 2, D, generator=g) * torch.tensor([1.0, 2.0 ** -30])[None, None, :, None] for _ in range(3)]
     rows[0][0, :, 1], rows[1][149, :, 1], rows[2][16:40, :, 1] = 0, 0, 0
     rows[2][16:40, :, 1, 0] = -0.0
-    check8(rows, torch.randn(3, H * G, D, generator=g).to(BF), page, 0.02)
+    check8(rows, torch.randn(3, H * G, D, generator=g).to(BF), page, 0.02, room)
 
 
-def test_e4m3_growing_values_and_scores():
-    """Scores and scales that grow along the sequence: bases move at every tile."""
+@pytest.mark.parametrize("H,G,D,page", SHAPES)
+@pytest.mark.parametrize("room", [0, 1 << 20], ids=["short_parts", "one_part"])
+def test_e4m3_growing_values_and_scores(H, G, D, page, room):
+    """Scores and scales that grow along the sequence, and that shrink: both bases move at every tile, in parts of few tiles and in one part of all."""
     g = torch.Generator().manual_seed(5)
-    H, G, D, n = 2, 4, 64, 260
+    n = 600
     q0 = torch.randn(1, H, 1, D, generator=g)
-    q = (q0 + 0.02 * torch.randn(2, H, G, D, generator=g)).reshape(2, H * G, D).to(BF)
-    rows = [torch.randn(n, H, 2, D, generator=g) for _ in range(2)]
+    q = (q0 + 0.02 * torch.randn(4, H, G, D, generator=g)).reshape(4, H * G, D).to(BF)
+    rows = [torch.randn(n, H, 2, D, generator=g) for _ in range(4)]
     step = torch.arange(n)[:, None, None] / n
-    for r, sign in zip(rows, (1, -1)):
-        r[:, :, 0] = sign * 40 * step * math.sqrt(D) * q0[0, :, 0] / q0[0, :, 0].square().sum(-1, keepdim=True)
-        r[:, :, 1] *= torch.exp2(60 * step)
-    check8(rows, q, 32, 1 / math.sqrt(D))
+    for r, score, value in zip(rows, (40, 40, -40, 0), (60, -40, 60, 60)):
+        r[:, :, 0] = 0.1 * r[:, :, 0] + score * step * math.sqrt(D) * q0[0, :, 0] / q0[0, :, 0].square().sum(-1, keepdim=True)
+        r[:, :, 1] *= torch.exp2(value * step)
+    check8(rows, q, page, 1 / math.sqrt(D), room)
 
 
 # ---- rings
