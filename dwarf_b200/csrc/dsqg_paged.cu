@@ -358,17 +358,21 @@ cudaError_t launch_step(const StepArgs& a, cudaStream_t s) {
 
 inline bool bad(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) != 0; }
 
-// The positions of a part: a multiple of 64, from the sizes alone.  Of blocks that run at once (`an_sm` per SM) about 85 % shall have work if lengths are spread
-// evenly up to the longest: below all of them, for one block too many takes as long as twice as many.  From 16 sequences on, which differ more, twice as many
-// parts.  Up to 2048 positions a part, up to 3200 where all blocks then run at once (55.4 us instead of 58.1 for 4 up to 100001, 4 x 8 heads in 8 bits; parts of
-// 2048 would be 564 blocks for 444 places: 64.8).  (us, with one part of the longest for every block that runs at once, whatever the lengths / with this: 16 sequences
-// up to 8192, 8 x 4 heads of 128 in 8 bits, 44 / 33; 4 up to 20000, 4 x 8 heads in 8 bits, 21.7 / 17.6; one of 4096, 8 x 4 heads in bf16, 10.5 / 7.6.)
+// The positions of a part: a multiple of 64, from the sizes alone.  Blocks run in waves of as many as the GPU holds at once (`an_sm` per SM), and one block too
+// many takes a wave of its own: about 85 % of one wave, or of two, three, .., shall have work if lengths are spread evenly up to the longest, in as few waves as keep
+// a part at 3200 positions or fewer: the longer the parts, the more is lost where lengths differ from that.  One wave against two, us, 4 x 8 heads of 128 in 8 bits,
+// lengths spread evenly / all equal: 8 sequences up to 30000 (parts of 1472 positions in one wave) 32.5 : 36.4 / 55.4 : 55.3, 4 up to 77000 (2048) 52.7 : 52.0 / 72.3 :
+// 67.6, 100001 (2688) 58.6 : 60.4 / 86.9 : 80.3, 125000 (3328) 74.2 : 70.5 / 108.6 : 95.7, 150000 (4032) 92.9 : 88.0 / 123.5 : 109.2; one of 131072, 8 x 8 heads in bf16
+// (2624), 85.0 : 88.8.  Three waves take more than two in all of these.
+// From 16 sequences on, which differ more, two waves, and parts of up to 2048 positions then (256 up to 2048, 8 x 4 heads of 64 in bf16, 83; a whole number of
+// waves of fewer positions, 88).
+// (us, with one part of the longest for every block that runs at once, whatever the lengths / with this: 16 sequences up to 8192, 8 x 4 heads of 128 in 8 bits, 44 /
+// 35; 4 up to 20000, 4 x 8 heads in 8 bits, 21.7 / 18.7; one of 4096, 8 x 4 heads in bf16, 10.5 / 7.7.)
 struct Split { int chunk, parts; };
 inline Split split_for(int S, int H, int G, int limit, int an_sm) {
-    const double pairs = (double)S * H * ((G + 15) / 16), share = (S + 1) / (2.0 * S), blocks = 148 * an_sm * 0.85 * (S < 16 ? 1 : 2);
     const long long most = ((long long)limit + 63) / 64;                       // in units of 64 positions
-    const double even = pairs * most * share / blocks;
-    long long units = (long long)std::ceil(S < 16 && even <= 50 ? even : std::min(even, 32.0));
+    const double pairs = (double)S * H * ((G + 15) / 16), share = (S + 1) / (2.0 * S), one_wave = pairs * most * share / (148 * an_sm * 0.85);
+    long long units = (long long)std::ceil(S < 16 ? one_wave / std::max(1.0, std::ceil(one_wave / 50.0)) : std::min(one_wave / 2, 32.0));
     const long long least = (most + 1023) / 1024;                              // no more than 1024 parts
     if (units < least) units = least;
     if (units < 1) units = 1;

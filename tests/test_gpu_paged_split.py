@@ -1,0 +1,38 @@
+"""How a paged step is cut into parts follows from the sizes and types; what comes out does not."""
+import math
+import random
+
+import pytest
+import torch
+
+import dwarf_b200
+from tests.serving_util import HALF, attention64
+from tests.test_gpu_paged import make_cache
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+BF, F, E4 = torch.bfloat16, torch.float32, torch.float8_e4m3fn
+
+
+@pytest.mark.parametrize("seed", range(40))
+def test_any_room(seed):
+    """Tables with room for 1 to 1,000,000 positions over the same sequences: scratch is enough for every plan, and parts of any length give the result."""
+    r = random.Random(seed)
+    dtype, q_dt = r.choice([(BF, BF), (E4, BF), (BF, BF), (E4, BF), (F, F), (E4, F), (BF, F)])
+    S, H, G, D, page = r.choice([1, 2, 5, 15, 16, 17]), r.choice([1, 2, 3]), r.choice([1, 2, 4, 8, 9, 17]), r.choice([32, 48, 64, 80, 96, 128, 40]), r.choice([16, 48, 64, 24])
+    lengths = [r.choice([0, 1, 63, 64, 65, 128, 129, r.randint(1, 300)]) for _ in range(S)]
+    g = torch.Generator().manual_seed(seed)
+    kv, ks, table, rows = make_cache(lengths, H, page, D, dtype, g)
+    q = torch.randn(S, H * G, D, generator=g).to(q_dt)
+    n = torch.tensor(lengths, dtype=torch.int32, device=DEV)
+    sc = 0.3 / math.sqrt(D)
+    for room in (1, 400, 3000, 30000, 200000, 1000000):
+        wide = torch.nn.functional.pad(table, (0, max(0, -(-room // page) - table.shape[1])), value=-1)
+        out = dwarf_b200.paged_attention_step(q.to(DEV), None, None, kv, wide, n, kv_scale=ks, scale=sc).double().cpu()
+        for s in range(S):
+            for h in range(H):
+                qs, x = q[s, h * G:(h + 1) * G].double(), rows[s][:, h]
+                o, spread, ds = attention64(qs, x[:, 0], x[:, 1], sc)
+                # operands in two 16-bit numbers: 2^-16, and what f16 leaves of the smallest
+                more = (2 * ds[:, None] + 2.0 ** -15 + (len(x) + 64) * 2.0 ** -24) * spread
+                assert ((out[s, h * G:(h + 1) * G] - o).abs() <= HALF[q_dt] * o.abs() + 1.01 * more).all(), (room, s, h)
