@@ -315,12 +315,18 @@ int dsqg_int4_linear(const void* x, const void* x_scale, const void* weight, con
     if (!x || !weight || !scales || !y || (dtype == DSQG_DTYPE_E4M3 && !x_scale)) return DSQG_ERR_NULL_POINTER;
     if (dtype != DSQG_DTYPE_BF16 && dtype != DSQG_DTYPE_E4M3) return DSQG_ERR_BAD_DTYPE;
     if (group != 32 && group != 64 && group != 128) return DSQG_ERR_UNSUPPORTED;
-    if (M < 1 || N < 1 || K < group || K % group || M > 65535 * 8) return DSQG_ERR_BAD_SHAPE;
+    if (M < 1 || N < 1 || K < group || K % group) return DSQG_ERR_BAD_SHAPE;
     if (bad(x) || bad(weight)) return DSQG_ERR_MISALIGNED;
-    const Int4Args a = {x, static_cast<const uint8_t*>(x_scale), static_cast<const uint8_t*>(weight), static_cast<const __nv_bfloat16*>(scales), bias,
-                        static_cast<__nv_bfloat16*>(y), M, N, K, K / group};
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
-    return cuda_status(dtype == DSQG_DTYPE_E4M3 ? launch_type<true>(a, group, s) : launch_type<false>(a, group, s));
+    constexpr int kRows = 65535 * 16;                          // of x, that a grid's second dimension has room for
+    for (long long m = 0; m < M; m += kRows) {
+        const int rows = (int)(M - m < kRows ? M - m : kRows);
+        const bool f8 = dtype == DSQG_DTYPE_E4M3;
+        const Int4Args a = {static_cast<const char*>(x) + m * K * (f8 ? 1 : 2), f8 ? static_cast<const uint8_t*>(x_scale) + m : nullptr, static_cast<const uint8_t*>(weight),
+                            static_cast<const __nv_bfloat16*>(scales), bias, static_cast<__nv_bfloat16*>(y) + m * N, rows, N, K, K / group};
+        if (cudaError_t e = f8 ? launch_type<true>(a, group, s) : launch_type<false>(a, group, s)) return cuda_status(e);
+    }
+    return DSQG_OK;
 }
 
 }  // extern "C"

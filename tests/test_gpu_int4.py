@@ -138,3 +138,15 @@ def test_refusals():
             bad()
     with pytest.raises(RuntimeError):
         f(x.requires_grad_(True), w, s)
+
+
+@pytest.mark.parametrize("e4m3", [False, True], ids=["bf16", "e4m3"])
+@pytest.mark.parametrize("M", [524_288, 524_289, 1_048_560, 1_048_563])
+def test_a_prompt_of_many_sequences(M, e4m3):
+    """As many rows as 256 prompts of 2048 tokens have, and more than one launch takes (65,535 blocks of 16)."""
+    x, xs, w, s, b, x64 = make(16, 32, 5, 32, e4m3)
+    y, size = oracle(x64, w, s, b)
+    at = torch.arange(M, device=DEV) * 7 % 16
+    out = dwarf_b200.int4_linear(x.to(DEV).view(torch.uint8)[at].view(x.dtype), w.to(DEV), s.to(DEV), b.to(DEV), x_scale=None if xs is None else xs.to(DEV).view(torch.uint8)[at].view(xs.dtype))
+    assert out.shape == (M, 5)
+    assert ((out.double() - y.to(DEV)[at]).abs() <= 2.0 ** -8 * y.abs().to(DEV)[at] + 40 * 2.0 ** -24 * size.to(DEV)[at]).all()      # 32 products, their scale, the bias
