@@ -315,7 +315,8 @@ int dsqg_int4_linear(const void* x, const void* x_scale, const void* weight, con
     if (!x || !weight || !scales || !y || (dtype == DSQG_DTYPE_E4M3 && !x_scale)) return DSQG_ERR_NULL_POINTER;
     if (dtype != DSQG_DTYPE_BF16 && dtype != DSQG_DTYPE_E4M3) return DSQG_ERR_BAD_DTYPE;
     if (group != 32 && group != 64 && group != 128) return DSQG_ERR_UNSUPPORTED;
-    if (M < 1 || N < 1 || K < group || K % group) return DSQG_ERR_BAD_SHAPE;
+    // a block's last row may be 255 beyond N, a warp's next tile eight of 512 columns beyond K
+    if (M < 1 || N < 1 || N > 0x7fffff00 || K < group || K > 0x7fffc000 || K % group) return DSQG_ERR_BAD_SHAPE;
     if (bad(x) || bad(weight)) return DSQG_ERR_MISALIGNED;
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     constexpr int kRows = 65535 * 16;                          // of x, that a grid's second dimension has room for

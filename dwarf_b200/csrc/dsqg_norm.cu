@@ -414,7 +414,8 @@ __global__ void __launch_bounds__(1024) dw_kernel(const float* __restrict__ part
 }
 
 inline bool bad(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) != 0; }
-inline bool bad_rows(long long rows, int D) { return rows < 1 || D < 1 || rows > 0x7fffffffLL || rows * D > 0x7fffffffffLL; }
+// A column index may go 1024 beyond a row.
+inline bool bad_rows(long long rows, int D) { return rows < 1 || D < 1 || D > 0x7ffff000 || rows > 0x7fffffffLL || rows * D > 0x7fffffffffLL; }
 inline bool bad_type(int t) { return t != DSQG_DTYPE_BF16 && t != DSQG_DTYPE_F32; }
 
 // Threads and pieces of a row, forward and backward: one piece a thread up to 2048 columns, two beyond, from 16,384 columns on four; wider than 32,768 a row

@@ -183,3 +183,16 @@ def test_int4_linear_keeps_its_values_through_casts():
     m.to(torch.bfloat16).half().float().double()
     for n, b in m.named_buffers():
         assert b.dtype == before[n].dtype and torch.equal(b, before[n])
+
+
+def test_sizes_next_to_the_last_int_are_refused(lib):
+    """A row's index arithmetic goes a little beyond its sizes: what would leave an int is not launched."""
+    f = dict(x=A, residual=None, weight=3 * A, y=5 * A, rstd=7 * A, rows=1, eps=1e-6, x_dtype=0, stream_dtype=0, y_dtype=0)
+    for D in (2 ** 31 - 1, 2 ** 31 - 8, 0x7ffff001):
+        p = _lib.RmsNorm(**f, D=D)
+        assert lib.dsqg_rms_norm_fwd(ctypes.byref(p), None) == -2
+        assert lib.dsqg_rms_norm_bwd(ctypes.byref(p), 8 * A, None, 9 * A, None, None, None, 0, None) == -2
+        assert lib.dsqg_rms_norm_bwd_scratch_bytes(1, D) == 0
+    assert lib.dsqg_rms_norm_bwd_scratch_bytes(1, 0x7ffff000) > 0
+    for N, K in ((2 ** 31 - 1, 32), (0x7fffff01, 32), (16, 2 ** 31 - 32), (16, 0x7fffc020)):
+        assert lib.dsqg_int4_linear(A, None, 2 * A, 3 * A, None, 4 * A, 1, N, K, 32, 0, None) == -2
