@@ -14,7 +14,7 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from .int4 import Int4Linear, Rows8
-from .modules import DSQGAttentionN_Fused, DSQGAttentionQW
+from .modules import DSQGAttentionN_Fused, DSQGAttentionQW, stock
 from .ops import OFFSETS_43, rms_norm, rms_norm_e4m3
 
 
@@ -35,6 +35,14 @@ class RMSNorm(nn.Module):
             return Rows8(y[0], y[1]), stream if branch is None else y[2]
         y = rms_norm(x, self.weight, residual, self.eps, out_dtype)
         return (y, stream) if branch is None else y
+
+
+def _add_norm(norm, branch, stream, rows8=False):
+    """norm.add, or the norm's own forward behind a sum of its own where somebody has replaced it or listens in on it."""
+    if stock(norm, RMSNorm):
+        return norm.add(branch, stream, rows8)
+    stream = stream if branch is None else stream + branch
+    return norm(stream), stream
 
 
 class FFN(nn.Module):
@@ -103,8 +111,9 @@ class Block(nn.Module):
 
 
 class CondMLM(nn.Module):
-    """fused_norms=True runs every norm together with the addition in front of it (`rms_norm`, one pass forward and one backward) instead of
-    F.rms_norm and a separate sum; under bf16 autocast the norm then leaves in bf16, which is what the projections behind it read.
+    """fused_norms=True has `forward` run every norm together with the addition in front of it (`rms_norm`, one pass forward and one backward) instead of
+    F.rms_norm and a separate sum; under bf16 autocast the norm then leaves in bf16, which is what the projections behind it read.  Blocks and norms that are
+    subclassed or wrapped, or have hooks, are called as they are.  (`prefill` runs as without; `decode_token` goes by prefill's cache_dtype.)
 
     attention = "condM": DSQG layers with the position bias only (the reference's condM,
     kernels/dsqg_attention_v2.py:434-477) -- the shape the end-to-end benchmark configuration names;
@@ -135,10 +144,15 @@ class CondMLM(nn.Module):
             half = torch.bfloat16 if torch.is_autocast_enabled("cuda") and torch.get_autocast_dtype("cuda") == torch.bfloat16 else None
             branch = None
             for blk in self.blocks:
-                y, x = blk.norm1.add(branch, x, out_dtype=half)
-                y, x = blk.norm2.add(blk.attn(y), x, out_dtype=half)
-                branch = blk.ffn(y)
-            return F.linear(self.norm.add(branch, x, out_dtype=half)[0], self.embedding.weight)
+                if stock(blk, Block) and stock(blk.norm1, RMSNorm) and stock(blk.norm2, RMSNorm):
+                    y, x = blk.norm1.add(branch, x, out_dtype=half)
+                    y, x = blk.norm2.add(blk.attn(y), x, out_dtype=half)
+                    branch = blk.ffn(y)
+                else:
+                    x, branch = blk(x if branch is None else x + branch), None
+            if stock(self.norm, RMSNorm):
+                return F.linear(self.norm.add(branch, x, out_dtype=half)[0], self.embedding.weight)
+            return F.linear(self.norm(x if branch is None else x + branch), self.embedding.weight)
         for blk in self.blocks:
             x = blk(x)
         return F.linear(self.norm(x), self.embedding.weight)       # tied lm_head
@@ -236,12 +250,12 @@ class CondMLM(nn.Module):
         for i, blk in enumerate(self.blocks):
             full = i not in state["ring_of"]
             reads = (blk.attn.qkv_proj,) if full else (blk.attn.qkv_proj, blk.attn.gate_proj)
-            h, x = blk.norm1.add(branch, x, rows8=all(type(p) is Int4Linear for p in reads))
+            h, x = _add_norm(blk.norm1, branch, x, rows8=all(stock(p, Int4Linear) for p in reads))
             branch = blk.attn.decode_paged(h, pages, state["page_of"][i]) if full else blk.attn.decode(h, cache, state["ring_of"][i], overlap=True)
-            h, x = blk.norm2.add(branch, x, rows8=type(blk.ffn.fc1) is Int4Linear)
+            h, x = _add_norm(blk.norm2, branch, x, rows8=stock(blk.ffn, FFN) and stock(blk.ffn.fc1, Int4Linear))
             branch = blk.ffn(h)
         state["t"] = t + 1
-        return F.linear(self.norm.add(branch, x)[0], self.embedding.weight)
+        return F.linear(_add_norm(self.norm, branch, x)[0], self.embedding.weight)
 
     @torch.no_grad()
     def generate(self, ids, max_new_tokens, temperature=0.0, generator=None, cache_dtype=None):

@@ -50,15 +50,16 @@ def _log_linear_bias(offsets, num_heads):
     return -logs[:, None] * alphas[None, :]
 
 
+def stock(m, cls):
+    """True when a module is of the class itself and nobody listens in on it (hooks) or has put another forward in its place: what it computes may then be part of
+    something larger."""
+    return type(m) is cls and "forward" not in m.__dict__ and not (m._forward_hooks or m._forward_pre_hooks or m._backward_hooks or m._backward_pre_hooks) \
+        and not torch.nn.modules.module._has_any_global_hook()
+
+
 def _plain(*mods):
-    """True when each of the modules is the stock class with fp32-style parameters and nobody listens in on it (hooks): its
-    forward may then be part of a larger native node."""
-    if torch.nn.modules.module._has_any_global_hook():
-        return False
-    for m, cls in mods:
-        if type(m) is not cls or "forward" in m.__dict__ or m._forward_hooks or m._forward_pre_hooks or m._backward_hooks or m._backward_pre_hooks or m.bias is None:
-            return False
-    return True
+    """True when each of the modules is the stock class with fp32-style parameters: its forward may then be part of a larger native node."""
+    return all(stock(m, cls) and m.bias is not None for m, cls in mods)
 
 
 class _DSQGAttentionBase(nn.Module):
