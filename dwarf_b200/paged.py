@@ -140,10 +140,8 @@ class PagedKVCache:
         self._reserve({s: self._length[s] + 1 for s in live})
         for s in live:
             self._length[s] += 1
-        if len(live) == len(self._length):
-            self.lengths.add_(1)
-        else:
-            self.lengths.copy_(torch.tensor(self._length, dtype=torch.int32))
+        # on the device, so that the host does not wait for the steps in flight
+        self.lengths.add_(1 if len(live) == len(self._length) else self.lengths > 0)
 
     def step(self, layer, q, k_new, v_new, scale=None, max_length: Optional[int] = None, out=None):
         """One new token per sequence against layer `layer` (see paged_attention_step); max_length defaults to the longest sequence, rounded up to whole

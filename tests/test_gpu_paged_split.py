@@ -36,3 +36,17 @@ def test_any_room(seed):
                 # operands in two 16-bit numbers: 2^-16, and what f16 leaves of the smallest
                 more = (2 * ds[:, None] + 2.0 ** -15 + (len(x) + 64) * 2.0 ** -24) * spread
                 assert ((out[s, h * G:(h + 1) * G] - o).abs() <= HALF[q_dt] * o.abs() + 1.01 * more).all(), (room, s, h)
+
+
+def test_advance_does_not_wait_for_the_gpu():
+    """A token within the pages at hand, with and without an empty slot of the batch: nothing is copied from the host."""
+    for counts in ([5, 0, 40], [5, 1, 40]):
+        c = dwarf_b200.PagedKVCache(1, 3, 1, 32, max_length=200, page_size=64, device=DEV)
+        c.extend(counts)
+        torch.cuda.set_sync_debug_mode("error")
+        try:
+            for _ in range(10):
+                c.advance()
+        finally:
+            torch.cuda.set_sync_debug_mode("default")
+        assert c.lengths.tolist() == [n + 10 if n else 0 for n in counts] == c._length
