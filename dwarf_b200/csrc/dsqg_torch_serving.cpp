@@ -216,7 +216,8 @@ Tensor paged_attention_step(const Tensor& q0, const std::optional<Tensor>& k0, c
     const int64_t limit = std::min(max_length.has_value() ? *max_length : room, room);
     if (limit < 0) throw py::value_error(w + ": max_length must not be negative");
     if (limit > 0x7fffff00) throw py::value_error(w + ": block_table covers too many positions");
-    if (softmax_scale.has_value() && !(*softmax_scale > 0 && *softmax_scale < 3e38)) throw py::value_error(w + ": scale must be positive and finite");
+    // in fp32, as the kernels take it: 0 there would stand for the default
+    if (softmax_scale.has_value() && !((float)*softmax_scale > 0.f && *softmax_scale < 3e38)) throw py::value_error(w + ": scale must be positive and finite in float32");
     const c10::cuda::CUDAGuard guard(kv.device());
     const Tensor q = rows_in(q0), k = rows_in(kn), v = rows_in(vn);
     Tensor out;

@@ -50,3 +50,18 @@ def test_advance_does_not_wait_for_the_gpu():
         finally:
             torch.cuda.set_sync_debug_mode("default")
         assert c.lengths.tolist() == [n + 10 if n else 0 for n in counts] == c._length
+
+
+def test_scales_at_the_ends_of_fp32():
+    """A scale that fp32 rounds to 0 is refused and not taken for the default; the smallest that it holds weighs all positions alike."""
+    g = torch.Generator().manual_seed(0)
+    for dtype, q_dt in ((BF, BF), (E4, BF), (F, F)):
+        kv, ks, table, rows = make_cache([40], 1, 16, 64, dtype, g)
+        q, n = torch.randn(1, 1, 64, generator=g).to(q_dt).to(DEV), torch.tensor([40], dtype=torch.int32, device=DEV)
+        for bad in (1e-60, 1e-46, 3.5e38):
+            with pytest.raises(ValueError):
+                dwarf_b200.paged_attention_step(q, None, None, kv, table, n, kv_scale=ks, scale=bad)
+        for small in (1e-30, 1e-44):
+            out = dwarf_b200.paged_attention_step(1e-3 * q, None, None, kv, table, n, kv_scale=ks, scale=small).double().cpu()
+            v = rows[0][:, 0, 1]
+            assert ((out[0, 0] - v.mean(0)).abs() <= HALF[q_dt] * v.mean(0).abs() + 1.01 * (2.0 ** -15 + 104 * 2.0 ** -24) * v.abs().mean(0)).all()
