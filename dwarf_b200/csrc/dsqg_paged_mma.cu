@@ -370,7 +370,7 @@ __global__ void __launch_bounds__(kWarps * 32, CTAS) step_mma_kernel(const StepA
                     l[n][e] += x[e];
                     if constexpr (F8) x[e] = exp2_fast(w[j][e]);
                 }
-                // Two operands of 16 bits, the number and what its rounding left: together off by 2^-16 of it (bf16) or 2^-22 (f16, see kTop).  One alone (2^-8 or
+                // Two operands of 16 bits, the number and what its rounding left: together off by 2^-15 of it (bf16) or 2^-22 (f16, see kTop).  One alone (2^-8 or
                 // 2^-11) is seen in the result: in bf16 0.0023 from 64 bits (2-norms, 64 sequences up to 4096, 8 x 4 heads of 128), where the result's own
                 // rounding to bf16 is 0.0017.
                 uint32_t hi, lo;
@@ -379,8 +379,9 @@ __global__ void __launch_bounds__(kWarps * 32, CTAS) step_mma_kernel(const StepA
                     const float2 held = __half22float2(*reinterpret_cast<const __half2*>(&hi));
                     lo = pack_f16x2(x[0] - held.x, x[1] - held.y);
                 } else {
-                    hi = pack_bf16x2(x[0], x[1]);
-                    lo = pack_bf16x2(x[0] - __uint_as_float(hi << 16), x[1] - __uint_as_float(hi & 0xffff0000u));
+                    // cut off and not rounded, so that nothing of it is negative, and never 0: an infinity in a value row is one in the result, and no NaN
+                    hi = __byte_perm(__float_as_uint(x[0]), __float_as_uint(x[1]), 0x7632);
+                    lo = pack_bf16x2(fmaxf(x[0] - __uint_as_float(hi << 16), 1.17549435e-38f), fmaxf(x[1] - __uint_as_float(hi & 0xffff0000u), 1.17549435e-38f));
                 }
                 pb[n][j] = transposed(hi); pl[n][j] = transposed(lo);
             }

@@ -23,7 +23,7 @@ def paged_bound(qs, r, sc, o, spread, ds, p_half):
 @pytest.mark.parametrize("H,G,D,page", [(2, 1, 32, 16), (1, 4, 128, 64), (2, 3, 96, 48), (1, 12, 64, 32), (1, 17, 128, 16), (2, 8, 80, 32), (1, 2, 48, 16)])
 @pytest.mark.parametrize("room", [0, 1 << 20], ids=["short_parts", "one_part"])
 def test_bf16_pages(H, G, D, page, room):
-    """bf16 keeps 2^-8 of a number and 2^-8 of what is left of it: 2^-16.  Scores near one another, so that their own error is far below, and values that
+    """bf16 cut off leaves up to 2^-7 of a number, and rounding that is off by 2^-8 of it: 2^-15.  Scores near one another, so that their own error is far below, and values that
     cancel, so that the result's rounding is too."""
     g = torch.Generator().manual_seed(D + G)
     lengths, sc = [1, 2, 20, 45, 300, 1000], 0.02
@@ -36,8 +36,28 @@ def test_bf16_pages(H, G, D, page, room):
         for h in range(H):
             qs, r = q[s, h * G:(h + 1) * G].double(), rows[s][:, h]
             o, spread, ds = attention64(qs, r[:, 0], r[:, 1], sc)
-            off, bound = (out[s, h * G:(h + 1) * G] - o).abs(), paged_bound(qs, r, sc, o, spread, ds, 2.0 ** -16)
+            off, bound = (out[s, h * G:(h + 1) * G] - o).abs(), paged_bound(qs, r, sc, o, spread, ds, 2.0 ** -15)
             assert (off <= bound).all(), (lengths[s], h, (off / bound).max())
+
+
+@pytest.mark.parametrize("H,G,D,page", [(2, 1, 32, 16), (1, 4, 128, 64), (1, 12, 64, 32), (1, 2, 48, 16), (1, 2, 64, 10)])
+@pytest.mark.parametrize("room", [0, 1 << 20], ids=["short_parts", "one_part"])
+def test_an_infinity_in_a_value_row_is_one_in_the_result(H, G, D, page, room):
+    """softmax v is infinite with the sign of v in the columns where one row is, whatever its probability is rounded to (1 and 1/2 leave nothing to round)."""
+    g = torch.Generator().manual_seed(D)
+    lengths = [1, 2, 40, 150]
+    kv, _, table, rows = make_cache(lengths, H, page, D, BF, g)
+    q = torch.randn(4, H * G, D, generator=g).to(BF)
+    for s, n in enumerate(lengths):
+        p, i = int(table[s, (n - 1) // page]), (n - 1) % page
+        kv[p, :, i, 1, 3], kv[p, :, i, 1, 5] = float("inf"), -float("inf")
+        if n == 2:
+            kv[p, :, :2, 0] = 0                                   # both scores are 0
+    table = torch.nn.functional.pad(table, (0, max(0, room // page - table.shape[1])), value=-1)
+    out = dwarf_b200.paged_attention_step(q.to(DEV), None, None, kv, table, torch.tensor(lengths, dtype=torch.int32, device=DEV), scale=0.02)
+    assert (out[:, :, 3] == float("inf")).all() and (out[:, :, 5] == -float("inf")).all()
+    rest = [d for d in range(D) if d not in (3, 5)]
+    assert torch.isfinite(out[:, :, rest]).all()
 
 
 def cache8(rows, page):
