@@ -166,11 +166,9 @@ class CondMLM(nn.Module):
             if g is None:
                 raise ValueError(f"quantize_weights: an input width of {n} is no multiple of 32")
             return Int4Linear.from_linear(linear, g)
-        for blk in self.blocks:
-            for m in (blk.attn, blk.ffn):
-                for name, child in list(m.named_children()):
-                    if type(child) is nn.Linear:
-                        setattr(m, name, convert(child))
+        linears = [(m, name, child) for blk in self.blocks for m in (blk.attn, blk.ffn) for name, child in m.named_children() if type(child) is nn.Linear]
+        for m, name, new in [(m, name, convert(child)) for m, name, child in linears]:       # none is replaced if one cannot be
+            setattr(m, name, new)
         return self
 
     # ---- incremental decoding over the O(1) DSQG rings -------------------------------------

@@ -196,3 +196,15 @@ def test_sizes_next_to_the_last_int_are_refused(lib):
     assert lib.dsqg_rms_norm_bwd_scratch_bytes(1, 0x7ffff000) > 0
     for N, K in ((2 ** 31 - 1, 32), (0x7fffff01, 32), (16, 2 ** 31 - 32), (16, 0x7fffc020)):
         assert lib.dsqg_int4_linear(A, None, 2 * A, 3 * A, None, 4 * A, 1, N, K, 32, 0, None) == -2
+
+
+def test_quantize_weights_changes_nothing_when_a_width_does_not_fit():
+    from dwarf_b200.model import CondMLM
+    m = CondMLM(vocab=11, dim=128, heads=2, layers=2, ffn=192, seq_len=32, full_attention_layer=1, offsets=(0, 1, 2))
+    before = dict(m.named_modules())
+    with pytest.raises(ValueError):
+        m.quantize_weights(128)                                   # fc2 has 192 columns
+    after = dict(m.named_modules())
+    assert before.keys() == after.keys() and all(after[n] is before[n] for n in before)
+    m.quantize_weights(64)
+    assert sum(type(x) is dwarf_b200.Int4Linear for x in m.modules()) == 2 * 2 + 3 + 2
