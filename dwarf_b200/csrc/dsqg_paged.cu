@@ -395,7 +395,6 @@ int page_args(const dsqg_pages* c, PageArgs* a) {
     if (bad(c->kv) || (reinterpret_cast<uintptr_t>(c->scale) & 1u)) return DSQG_ERR_MISALIGNED;
     a->kv = static_cast<char*>(c->kv); a->scale = static_cast<uint8_t*>(c->scale); a->table = c->table;
     a->dtype = c->dtype; a->pages = c->pages; a->page = c->page_size; a->columns = c->columns; a->H = c->heads; a->D = c->D; a->S = c->sequences;
-    a->row_bytes = c->D * (c->dtype == DSQG_DTYPE_F32 ? 4 : c->dtype == DSQG_DTYPE_BF16 ? 2 : 1);
     return DSQG_OK;
 }
 

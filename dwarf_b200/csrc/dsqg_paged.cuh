@@ -12,7 +12,6 @@ namespace dsqg {
 struct PageArgs {
     char* kv; uint8_t* scale; const int32_t* table;
     int dtype, pages, page, columns, H, D, S;
-    int row_bytes;             // of a key or value row
 
     // Index of the first row of a page for head h, -1 where the table names no page of the cache: nothing is read or written there.
     __device__ __forceinline__ long long rows_of(int s, int h, int column) const {
@@ -43,7 +42,7 @@ __device__ __forceinline__ Range range_of(const StepArgs& a, int s, int part) {
     return r;
 }
 
-// The new token's key and value as the cache holds them, by the 32 lanes of a warp: to `row` ([2][row_bytes] in shared memory, its scale bytes at
+// The new token's key and value as the cache holds them, by the 32 lanes of a warp: to `row` ([2][D] in shared memory, its scale bytes at
 // `bytes`) and, where `store` says so, to the cache.  D <= 128.
 __device__ __forceinline__ void new_row(const StepArgs& a, int s, int h, int position, bool store, char* row, uint8_t* bytes) {
     const PageArgs& c = a.c;
