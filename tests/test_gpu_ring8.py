@@ -160,3 +160,41 @@ def test_refusals():
         c.prefill(0, x, x.bfloat16())
     with pytest.raises(ValueError):
         c.prefill(0, x.cpu(), x.cpu())
+
+
+@pytest.mark.parametrize("S,H,D", [(3, 2, 32), (2, 3, 64), (2, 1, 128), (3, 1, 48), (2, 2, 8), (2, 1, 40), (2, 1, 120)])
+@pytest.mark.parametrize("name", list(SETS))
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("overlap", [False, True])
+def test_slots_that_are_no_tap_hold_nan(S, H, D, name, dt, overlap):
+    """Every width, type, form and number of passes: rows of NaN in all slots but the live taps change nothing, and stay where they are."""
+    offsets = SETS[name]
+    R = max(offsets) + 1 + (name == "one")
+    g = torch.Generator().manual_seed(S * 100 + D)
+    kv, ks = rings(S, H, R, D, g)
+    q, kn, vn = (torch.randn(S, H, D, generator=g).to(dt).to(DEV) for _ in range(3))
+    head = torch.randint(0, R, (S,), generator=g, dtype=torch.int32)
+    fill = torch.randint(1, R + 1, (S,), generator=g, dtype=torch.int32)
+    fill[0], fill[1] = R, 1
+    pb = torch.randn(len(offsets), H, generator=g).to(DEV)
+    dead = torch.ones(S, R, dtype=torch.bool)
+    for s in range(S):
+        for o in offsets:
+            if o < fill[s]:
+                dead[s, (head[s] - o) % R] = False
+    dead = dead.to(DEV)[:, None].expand(S, H, R)
+    for se in (None, 0.1 * torch.randn(len(offsets), D, generator=g).to(DEV)):
+        runs = []
+        for poison in (False, True):
+            kv1, ks1 = kv.clone(), ks.clone()
+            if poison:
+                kv1.view(torch.uint8)[dead], ks1.view(torch.uint8)[dead] = 0x7f, 255
+            before, before_s = kv1.view(torch.uint8).clone(), ks1.view(torch.uint8).clone()
+            out = dwarf_b200.dsqg_decode_step_kv(q, kn, vn, kv1, head.to(DEV), pb, None, se, offsets, fill.to(DEV), overlap=overlap, kv_scale=ks1)
+            at = (torch.arange(S), slice(None), head.long())
+            new, new_s = quantize64(torch.stack([kn, vn], 2))
+            assert torch.equal(kv1[at].float().double().cpu(), new) and torch.equal(scale_values(ks1[at]), new_s)
+            kv1.view(torch.uint8)[at], ks1.view(torch.uint8)[at] = before[at], before_s[at]
+            assert torch.equal(kv1.view(torch.uint8), before) and torch.equal(ks1.view(torch.uint8), before_s)
+            runs.append(out)
+        assert torch.isfinite(runs[1]).all() and torch.equal(runs[0], runs[1])
