@@ -126,3 +126,41 @@ def test_refusals():
     with pytest.raises(TypeError):
         with torch.no_grad():
             m.prefill(ids_of(1, 8), cache_dtype=torch.float16)
+
+
+@pytest.mark.parametrize("attention,full", [("condU", 1), ("condM", 0)])
+@pytest.mark.parametrize("dtype,bits4", [(torch.bfloat16, False), (torch.float8_e4m3fn, False), (torch.float8_e4m3fn, True)], ids=["bf16", "e4m3", "e4m3_int4"])
+def test_a_bf16_model_serves(attention, full, dtype, bits4):
+    """The documented serving model: bf16 parameters throughout, fused norms.  Its decode path against its whole prefix: both round every activation to bf16 (2^-8, some 20 in a row
+    and in three layers, 2e-2 as above and as much again for what differs in order), with 8-bit caches and norms as above."""
+    m = model(attention, full=full, fused_norms=True).to(torch.bfloat16).eval()
+    if bits4:
+        m.quantize_weights()
+    S, prompt, new = 3, 70, 12
+    ids = ids_of(S, prompt + new)
+    with torch.no_grad():
+        whole = m(ids)
+        assert whole.dtype is torch.bfloat16
+        logits, state = m.prefill(ids[:, :prompt], max_len=prompt + new, cache_dtype=dtype, page_size=16)
+        assert off(logits, whole[:, prompt - 1]) < 4e-2
+        for t in range(prompt, prompt + new):
+            logits = m.decode_token(ids[:, t], state)
+            assert logits.dtype is torch.bfloat16 and off(logits, whole[:, t]) < (0.2 if bits4 else 0.15 if dtype is torch.float8_e4m3fn else 4e-2), f"position {t}"
+    a, b = m.generate(ids[:, :prompt], 6, cache_dtype=dtype), m.generate(ids[:, :prompt], 6, cache_dtype=dtype)
+    assert a.shape == (S, prompt + 6) and torch.equal(a, b)
+
+
+def test_a_bf16_model_trains_with_fused_norms():
+    """bf16 parameters: the same roundings of every activation in both, but for the sums of a norm.  Where bf16 rounds one the other way the two part by 2^-8 of it: 4e-2 as above for
+    the result, five times that for gradients."""
+    plain, fused = model("condU").to(torch.bfloat16), model("condU", fused_norms=True).to(torch.bfloat16)
+    ids, got = ids_of(2, 60), []
+    for m in (plain, fused):
+        y = m(ids)
+        y.float().square().mean().backward()
+        got.append([y.detach()] + [p.grad.clone() for p in m.parameters()])
+    assert off(got[1][0], got[0][0]) < 4e-2
+    for a, b, (name, p) in zip(got[1][1:], got[0][1:], plain.named_parameters()):
+        assert a.dtype is p.dtype
+        if b.norm() > 1e-2 * max(g.norm() for g in got[0][1:]):
+            assert off(a, b) < 0.2, name
