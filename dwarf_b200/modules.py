@@ -53,7 +53,8 @@ def _log_linear_bias(offsets, num_heads):
 def stock(m, cls):
     """True when a module is of the class itself and nobody listens in on it (hooks) or has put another forward in its place: what it computes may then be part of
     something larger."""
-    return type(m) is cls and "forward" not in m.__dict__ and not (m._forward_hooks or m._forward_pre_hooks or m._backward_hooks or m._backward_pre_hooks) \
+    d = m.__dict__                                             # asked for some 40 modules a token
+    return type(m) is cls and not (d["_forward_hooks"] or d["_forward_pre_hooks"] or d["_backward_hooks"] or d["_backward_pre_hooks"] or "forward" in d) \
         and not torch.nn.modules.module._has_any_global_hook()
 
 
