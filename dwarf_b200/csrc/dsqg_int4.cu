@@ -9,8 +9,9 @@
 // inside one group of 32 columns, so a group's products are summed unscaled and its scale is applied to the fp32 sum.  x goes straight to registers,
 // 128 columns ahead of its use (it is small and stays in L1), the scales a tile ahead.
 //
-// What bounds it is unpacking, not memory: 1 x 4096 x 16384 takes 12.2 us where the copies alone take 6 (HBM's floor 5.3), at some 180 instructions for 16
-// rows of 128 columns, half of them on the pipe of shifts and logic that takes two cycles for each.  Built and taken back: x brought to f16 and into the
+// What bounds it is waiting: 1 x 4096 x 16384 takes 12.2 us where the copies alone take 6 (HBM's floor 5.3), with the issue slots at 52 %, the pipe of shifts and
+// logic at 51 % (some 180 instructions for 16 rows of 128 columns, half of them there), DRAM at 28 % and a fifth of the warps there could be: a warp has 3.5
+// tiles, one ahead, behind a first copy that nothing hides.  Where N is small it is also few blocks (64 of them for 1 x 8192 x 1024, 4.7 us, floor 0.7).  Built and taken back: x brought to f16 and into the
 // order of the pairs in shared memory, with the columns of a row block shared out over a cluster (11.5, but 3.3 instead of 2.3 us for 1 x 256 x 768 and
 // 9.5 instead of 7.7 for 8 x 8192 x 4096); four warps a block (13.5); 64-byte pieces of eight rows a copy (18.4); scales fetched 128 columns ahead (16.4).
 #include "dsqg_rows8.cuh"

@@ -149,8 +149,8 @@ template <bool WRITE, int HC> cudaError_t launch_move(const MoveArgs& a, cudaStr
         default: return launch_after(move_kernel<16, HC, WRITE>, blocks, kT, 0, s, a);
     }
 }
-// Heads a group: three where they divide up evenly, two otherwise (us, write and read back of 6820 tokens, 12 heads of 64, 8 bits: one 11.4 and 8.9, two 10.6 and
-// 8.2, three 10.0 and 7.7, four 12.5 and 9.6; read of 7800 tokens, 8 heads of 128: two 22.5, three 24.3, four 25.5).
+// Heads a group: three where they divide up evenly, two otherwise (us, write and read back of 6820 tokens, 12 heads of 64, 8 bits: one 9.8 and 8.6, two 9.5 and
+// 7.7, three 9.0 and 7.2, four 9.5 and 9.2; read of 14,501 tokens, 8 heads of 128: one 21.3, two 21.9, three 23.8, four 24.3; floor 13.6).
 template <bool WRITE> cudaError_t launch_move_heads(const MoveArgs& a, cudaStream_t s) {
     return a.c.H == 1 ? launch_move<WRITE, 1>(a, s) : a.c.H % 3 == 0 ? launch_move<WRITE, 3>(a, s) : launch_move<WRITE, 2>(a, s);
 }

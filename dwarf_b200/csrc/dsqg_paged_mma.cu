@@ -15,8 +15,8 @@
 // each column that follows the largest of these sums, so that what is largest in the result is largest in f16, whatever scales other rows have.  (Relative to the
 // largest scale alone, a value row 2^20 above the others took the bits of all that came with or after it, even one that no query looks at.)
 //
-// (Keys in 8 bits as they lie, through m16n8k32 with e4m3 operands and the query as two e4m3 numbers: 61 us instead of 58 for 4 sequences of 100001
-// positions.  Query heads as the 16 rows of the product instead: half of every accumulator idle up to 8 heads, 179 registers, 8 warps an SM and 636 instructions a
+// (Keys in 8 bits as they lie, through m16n8k32 with e4m3 operands and the query as two e4m3 numbers, when a probability was one number: 61 us instead of 58 for
+// 4 sequences of 100001 positions.  Query heads as the 16 rows of the product instead: half of every accumulator idle up to 8 heads, 179 registers, 8 warps an SM and 636 instructions a
 // tile of 8-bit rows of 128 columns; 160 us for 4 sequences of 100001 positions, 4 x 8 heads.)
 //
 // mma.sync and not tcgen05: an operand of 128 rows would be at most an eighth full (query heads of one key-value head), and what is in question is memory.
@@ -470,8 +470,8 @@ template <int D, bool F8, int HT, int STAGES, int CTAS> cudaError_t launch_one(c
 }
 template <int D, bool F8> cudaError_t launch_width(const StepArgs& a, cudaStream_t s) {
     // Two CTAs of four warps and 8-KB tiles in bf16, three in 8 bits, four up to 96 columns, two tiles ahead each: 88 us for 64 sequences up to 4096, 8 x 4 heads
-    // of 128 in bf16 (84 at the rate of a copy), 55.4 us for 4 up to 100001, 4 x 8 heads of 128 in 8 bits (44).  Four CTAs in 8 bits: 17.7 -> 19.0 for 4 up to 20000,
-    // 33.1 -> 33.9 for 16 up to 8192; three at 80 columns 31.7 -> 32.7.  Three tiles ahead: the same.  bf16 with three CTAs and one tile ahead 1 % more, two tiles
+    // of 128 in bf16 (84 at the rate of a copy), 55 us for 4 up to 100001, 4 x 8 heads of 128 in 8 bits (44).  With one number a probability, four CTAs in 8 bits: 17.7 -> 19.0
+    // for 4 up to 20000, 33.1 -> 33.9 for 16 up to 8192; three at 80 columns 31.7 -> 32.7.  Three tiles ahead: the same.  bf16 with three CTAs and one tile ahead 1 % more, two tiles
     // a round 14 % more in 8 bits; tiles by the copy engine through a swizzled tensor map 2 % more in bf16 and 2 % less in 8 bits.
     if (a.G > 8) return launch_one<D, F8, 2, 3, 2>(a, s);
     return launch_one<D, F8, 1, 3, (!F8 ? 2 : D > 96 ? 3 : 4)>(a, s);

@@ -404,7 +404,7 @@ int dsqg_ring_prefill(const void* k, const void* v, void* k_ring, void* v_ring,
 /* Root-mean-square norm of a residual stream, the addition in front of it included:
  *     h = x + residual (rounded to stream_dtype), y = h / sqrt(mean(h^2) + eps) * weight.
  * x, residual: bf16 or fp32 [rows,D], each its own type; residual nullable: h = x, which is not written.  y: bf16, fp32 or e4m3 with y_scale
- * [rows].  rstd [rows] fp32 (nullable): 1 / sqrt(..), for the backward pass.  Any D >= 1; tensors start on 16 bytes and are read in pieces of eight
+ * [rows].  rstd [rows] fp32 (nullable): 1 / sqrt(..), for the backward pass.  D from 1 to 2^31 - 4096; tensors start on 16 bytes and are read in pieces of eight
  * elements, of which two rows share one where D is no multiple of 8.  h may be residual or x where the types allow it. */
 typedef struct dsqg_rms_norm {
     const void* x; const void* residual; const float* weight;
@@ -455,7 +455,7 @@ int dsqg_paged_step(const dsqg_pages* cache, const void* q, const void* k_new, c
 
 /* y [M,N] bf16 = x [M,K] W^T + bias, W[n,k] = (nibble - 8) * scales[n, k / group]: weight [N,K/2] bytes, the nibble of an even k in the low half;
  * scales bf16 [N,K/group], group 32, 64 or 128, K a multiple of it; bias fp32 [N], nullable.  x: bf16, or e4m3 with x_scale [M] bytes.  fp32 sums; made
- * for a few rows (a decode step): 16 rows at a time read the weights once. */
+ * for a few rows (a decode step): 16 rows at a time read the weights once.  Any M >= 1; N up to 2^31 - 256, K up to 2^31 - 16384. */
 int dsqg_int4_linear(const void* x, const void* x_scale, const void* weight, const void* scales, const float* bias, void* y, int M, int N, int K, int group, int dtype,
                      void* stream);
 
