@@ -36,7 +36,7 @@ def paged_attention_step(q, k_new, v_new, kv_pages, block_table, lengths, kv_sca
     i // (Hq / H)) -> [S,Hq,D].
 
     lengths int32 [S] on the device counts the new token: k_new, v_new [S,H,D] are stored at position lengths[s] - 1 and attended to as stored
-    (None, None: nothing is stored, all lengths[s] positions are read).  A length of 0 gives zeros and stores nothing.  max_length: no length is
+    (None, None: nothing is stored, all lengths[s] positions are read).  Sequences may share pages that no token is stored in.  A length of 0 gives zeros and stores nothing.  max_length: no length is
     above it (default: what the table has room for); a longer one gives NaN, and so does a position for which the table names no page.  The
     cache's length is split over the GPU by max_length, so a tight bound is faster for few sequences.  scale: of the scores, positive in fp32, default
     1/sqrt(D).  Sums are held in fp32; on tensor cores a probability enters the product with the values as two 16-bit numbers, off by 2^-15 of it over bf16

@@ -446,7 +446,7 @@ int dsqg_paged_write(const dsqg_pages* cache, const void* k, const void* v, long
 int dsqg_paged_read(const dsqg_pages* cache, void* k, void* v, const int32_t* cu_seqlens, const int32_t* start, long long tokens, int dtype, void* stream);
 /* One new token per sequence: out[s,i] = softmax(scale q[s,i] . K^T) V over the lengths[s] positions of sequence s, for query heads i of key-value head
  * i / (q_heads / heads).  q, out [sequences,q_heads,D], k_new, v_new [sequences,heads,D] in dtype (bf16 or fp32).  With k_new, v_new (both or
- * neither) the token at position lengths[s] - 1 is stored first and attended to as stored.  lengths int32 [sequences], 0 <= lengths[s] <= max_length <=
+ * neither) the token at position lengths[s] - 1 is stored first and attended to as stored; sequences may share pages that no token is stored in.  lengths int32 [sequences], 0 <= lengths[s] <= max_length <=
  * columns * page_size: 0 gives zeros and stores nothing, a length outside gives NaN.  Long sequences are split and joined (scratch; the order of the
  * sums follows from the sizes, max_length among them, and from the sequence's own length).  scale <= 0: 1/sqrt(D). */
 size_t dsqg_paged_step_scratch_bytes(int sequences, int heads, int q_heads, int D, int max_length);
