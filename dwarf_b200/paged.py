@@ -36,11 +36,14 @@ def paged_attention_step(q, k_new, v_new, kv_pages, block_table, lengths, kv_sca
     i // (Hq / H)) -> [S,Hq,D].
 
     lengths int32 [S] on the device counts the new token: k_new, v_new [S,H,D] are stored at position lengths[s] - 1 and attended to as stored
-    (None, None: nothing is stored, all lengths[s] positions are read).  Sequences may share pages that no token is stored in.  A length of 0 gives zeros and stores nothing.  max_length: no length is
-    above it (default: what the table has room for); a longer one gives NaN, and so does a position for which the table names no page.  The
-    cache's length is split over the GPU by max_length, so a tight bound is faster for few sequences.  scale: of the scores, positive in fp32, default
-    1/sqrt(D).  Sums are held in fp32; on tensor cores a probability enters the product with the values as two 16-bit numbers, off by 2^-15 of it over bf16
-    pages and by 2^-22 over 8-bit pages (2^-33 of the largest term where it is that small).  Fastest with bf16 queries over bf16 or 8-bit pages of a multiple of 16 positions, D a multiple of 32, 48 or 80."""
+    (None, None: nothing is stored, all lengths[s] positions are read).  Sequences may share pages that no token is stored in.  A length of 0
+    gives zeros and stores nothing.  max_length: no length is above it (default: what the table has room for); a longer one gives NaN, and so
+    does a position for which the table names no page.  The cache's length is split over the GPU by max_length, so a tight bound is faster for
+    few sequences.  scale: of the scores, positive in fp32, default 1/sqrt(D).
+
+    Sums are held in fp32; on tensor cores a probability enters the product with the values as two 16-bit numbers, off by 2^-15 of it over bf16
+    pages and by 2^-22 over 8-bit pages (2^-33 of the largest term where it is that small).  Fastest with bf16 queries over bf16 or 8-bit pages
+    of a multiple of 16 positions, D a multiple of 32, 48 or 80."""
     return _lib.native().paged_attention_step(q, k_new, v_new, kv_pages, block_table, lengths, kv_scale, scale, max_length, out)
 
 
