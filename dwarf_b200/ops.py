@@ -58,9 +58,10 @@ def causal_mean(x):
 def rms_norm(x, weight, residual=None, eps=1e-6, out_dtype=None):
     """Root-mean-square norm, the residual's addition in front of it included: h = x + residual in residual's type, y = h / sqrt(mean(h^2) + eps) *
     weight over the last dimension.  x, residual bf16 or fp32 [..., D], each its own type (a bf16 branch onto an fp32 stream); weight [D];
-    out_dtype: bf16 or fp32, default that of the stream.  Returns y, or (y, h) with a residual.  One pass over memory; differentiable in all
-    three tensors (the pre-norm blocks of the benchmark model, `x = x + f(x); norm(x)`), once.  As with any operator of PyTorch, a backward pass
-    is captured into a graph only after warming up on a side stream, with no eager graph of the same leaves alive."""
+    out_dtype: bf16 or fp32, default that of the stream.  Returns y, or (y, h) with a residual.  Squares are summed in fp32, as F.rms_norm does:
+    elements of h from 1.8e19 on make a row of y 0.  One pass over memory; differentiable in all three tensors (the pre-norm blocks of the
+    benchmark model, `x = x + f(x); norm(x)`), once.  As with any operator of PyTorch, a backward pass is captured into a graph only after
+    warming up on a side stream, with no eager graph of the same leaves alive."""
     y, h = _lib.native().rms_norm(x, weight, residual, eps, out_dtype)
     return y if residual is None else (y, h)
 

@@ -403,6 +403,7 @@ int dsqg_ring_prefill(const void* k, const void* v, void* k_ring, void* v_ring,
 
 /* Root-mean-square norm of a residual stream, the addition in front of it included:
  *     h = x + residual (rounded to stream_dtype), y = h / sqrt(mean(h^2) + eps) * weight.
+ * Squares are summed in fp32: elements of h from 1.8e19 on make a row 0.
  * x, residual: bf16 or fp32 [rows,D], each its own type; residual nullable: h = x, which is not written.  y: bf16, fp32 or e4m3 with y_scale
  * [rows].  rstd [rows] fp32 (nullable): 1 / sqrt(..), for the backward pass.  D from 1 to 2^31 - 4096; tensors start on 16 bytes and are read in pieces of eight
  * elements, of which two rows share one where D is no multiple of 8.  h may be residual or x where the types allow it. */
